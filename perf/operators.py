@@ -4,7 +4,7 @@
               or per sample, a token's row;
 * ``grad``    the gradient of that table (``landmark_b200.embedding.embedding_backward``): the output's rows summed by
               index, every row of the table written;
-* ``adamw``   one AdamW step over many tensors at once (``landmark_b200.optim.adamw_step``), with states in 32 bits or in
+* ``adamw``   one AdamW step over many tensors at once (``landmark_b200.optim.AdamWTensors``), with states in 32 bits or in
               blocks of 8-bit codes.
 
 ``run`` computes each either in elementary torch operations (``own`` false) or through the package.
@@ -208,7 +208,7 @@ def prepare(case, seed):
 
 def _run_own(s):
     from landmark_b200.embedding import embedding, embedding_backward
-    from landmark_b200.optim import adamw_step
+    from landmark_b200.optim import AdamWTensors
 
     c = s["case"]
     if c["op"] == "lookup":
@@ -218,8 +218,9 @@ def _run_own(s):
             return embedding_backward(s["grad"], s["indices"], c["rows"], scale=c["scale"], out=s["into"], accumulate=True)
         return embedding_backward(s["grad"], s["indices"], c["rows"], scale=c["scale"], dtype=DTYPES[c["out"]])
     w = s["views"]
-    adamw_step(w["p"], w["g"], w["m"], w["v"], step=s["step"], lr=c["lr"], betas=(c["beta1"], c["beta2"]), eps=1e-8, weight_decay=c["decay"],
-               exp_avg_scales=w.get("ms"), exp_avg_sq_scales=w.get("vs"), masters=w.get("master"), seed=s["seed"])
+    if "tensors" not in s:  # a trainer's parameters and states, checked when it starts
+        s["tensors"] = AdamWTensors(w["p"], w["m"], w["v"], w.get("ms"), w.get("vs"), w.get("master"))
+    s["tensors"].step(w["g"], step=s["step"], lr=c["lr"], betas=(c["beta1"], c["beta2"]), eps=1e-8, weight_decay=c["decay"], seed=s["seed"])
 
 
 # -- plain forms -----------------------------------------------------------------------------------------------------------
