@@ -427,6 +427,47 @@ int gnr_composite_rgb(GnrModel* m, int64_t n_rays, int white_bg, void* workspace
                       int64_t max_valid, int64_t max_app, int n_samples, const float* rgb_samples, int64_t n_rgb,
                       float* rgb_map, float* depth_map, void* stream);
 
+/* ---- What a model learns: embedding rows, their gradient, optimiser steps ---------------------------------------------
+ * These entries need no model; they work on the current CUDA device, which has to be the one of the pointers and the stream.
+ * Element types of tables, gradients and parameters: */
+enum { GNR_FP32 = 0, GNR_FP16 = 1, GNR_BF16 = 2 };
+
+/* out[t] = round(scale * table[indices[t]]), rows of ``dim`` values, ``*_stride`` values apart (at least ``dim``); the product
+ * in fp32, rounded once to ``type``.  A negative index is a masked place: its row is zeros.  An index of ``rows`` or more is an
+ * error that only the device sees: its row is NaN.  ``index_bits`` 32 or 64.  (The appearance latent of every sample,
+ * compute_app_latent, app/models/gridnerf_sequential.py:429-437.) */
+int gnr_embedding_lookup(const void* table, int type, int64_t rows, int dim, int64_t table_stride, const void* indices,
+                         int index_bits, int64_t n, float scale, void* out, int64_t out_stride, void* stream);
+/* Its gradient: out[v] = round(scale * sum of grad[t] over the t with indices[t] == v), for every row v of ``rows``; with
+ * ``accumulate`` added to what out holds (rows that no index names are then not touched).  Sums in fp32, in an order that only
+ * the inputs decide.  Masked places, indices past the table and those equal to ``padding_row`` (-1: none) are left out, their
+ * rows of ``grad`` not read.  ``workspace`` on a 16-byte boundary, its contents are scratch. */
+int gnr_embedding_grad_workspace_bytes(int64_t n, int64_t rows, int dim, size_t* bytes_h);
+int gnr_embedding_grad(const void* grad, int grad_type, int dim, int64_t grad_stride, const void* indices, int index_bits,
+                       int64_t n, int64_t rows, int64_t padding_row, float scale, int accumulate, void* out, int out_type,
+                       int64_t out_stride, void* workspace, size_t workspace_bytes, void* stream);
+
+/* One tensor of an optimiser step; all pointers are device pointers to dense arrays of ``n`` values (scales: of
+ * ceil(n / GNR_ADAMW_BLOCK)). */
+enum { GNR_ADAMW_BLOCK = 256 }; /* values that share the scales of the 8-bit states */
+typedef struct GnrAdamwTensor {
+  void* param;
+  const void* grad;
+  void* exp_avg;           /* fp32, or e4m3 codes c of the first moment scale * c                        */
+  void* exp_avg_sq;        /* fp32, or e4m3 codes c of the second moment (scale * c)^2                   */
+  float* exp_avg_scale;    /* 8-bit states only                                                          */
+  float* exp_avg_sq_scale;
+  float* master;           /* null, or the parameter in fp32 (``param`` is then its rounded image)       */
+  int64_t n;
+  int64_t number;          /* tells tensors apart in the random rounding of the 8-bit states             */
+} GnrAdamwTensor;
+/* One AdamW step (decoupled weight decay) over all of them, for tensors of one parameter type and one gradient type:
+ *   m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2,
+ *   p = p (1 - lr weight_decay) - lr / (1 - beta1^step) m / (sqrt(v / (1 - beta2^step)) + eps),
+ * in fp32.  ``state_bits`` 32 or 8; ``step`` counts from 1.  ``tensors_h`` is read before the call returns. */
+int gnr_adamw_step(const GnrAdamwTensor* tensors_h, int n_tensors, int param_type, int grad_type, int state_bits, int64_t step,
+                   double lr, double beta1, double beta2, double eps, double weight_decay, uint32_t seed, void* stream);
+
 /* Per-stage timing with CUDA events recorded on the launching stream around every stage of
  * gnr_render_chunk / gnr_render_host (the counterpart of the reference's PipeStagesProfiler,
  * dist_render/comm/profiler.py:18-69, at kernel granularity).  gnr_profile_collect waits for

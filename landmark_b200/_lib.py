@@ -13,6 +13,8 @@ _PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_PKG, "libgridnerf_b200.so")
 
 STAGE_NAMES = ("sample", "compact", "density", "weights", "compact_app", "app_gather", "mlp", "composite")
+FP32, FP16, BF16 = 0, 1, 2  # element types of the training entries
+ADAMW_BLOCK = 256  # GNR_ADAMW_BLOCK
 SAMPLE_STATIC_SCRATCH_BYTES = (4 << 20) + 4096
 MAX_LANES = 8  # GNR_MAX_LANES
 EXPIRE_ANY, EXPIRE_PROJECTION, EXPIRE_NETWORK = 1, 2, 3  # gnr_debug_wait
@@ -47,6 +49,20 @@ class GnrConfig(C.Structure):
         ("den_storage", C.c_int32),
         ("unfused_appearance", C.c_int32),
         ("reserved", C.c_int32 * 3),
+    ]
+
+
+class GnrAdamwTensor(C.Structure):
+    _fields_ = [
+        ("param", C.c_void_p),
+        ("grad", C.c_void_p),
+        ("exp_avg", C.c_void_p),
+        ("exp_avg_sq", C.c_void_p),
+        ("exp_avg_scale", C.c_void_p),
+        ("exp_avg_sq_scale", C.c_void_p),
+        ("master", C.c_void_p),
+        ("n", C.c_int64),
+        ("number", C.c_int64),
     ]
 
 
@@ -109,6 +125,11 @@ SIGNATURES = {
     "gnr_app_features_points": (_INT, [_P, _P, _I64, _P, _SZ, _P, _P]),
     "gnr_mlp_features": (_INT, [_P, _P, _P, _I64, _P, _SZ, _P, _P]),
     "gnr_composite_rgb": (_INT, [_P, _I64, _INT, _P, _SZ, _I64, _I64, _INT, _P, _I64, _P, _P, _P]),
+    "gnr_embedding_lookup": (_INT, [_P, _INT, _I64, _INT, _I64, _P, _INT, _I64, C.c_float, _P, _I64, _P]),
+    "gnr_embedding_grad_workspace_bytes": (_INT, [_I64, _I64, _INT, C.POINTER(_SZ)]),
+    "gnr_embedding_grad": (_INT, [_P, _INT, _INT, _I64, _P, _INT, _I64, _I64, _I64, C.c_float, _INT, _P, _INT, _I64, _P, _SZ, _P]),
+    "gnr_adamw_step": (_INT, [_P, _INT, _INT, _INT, _INT, _I64, C.c_double, C.c_double, C.c_double, C.c_double, C.c_double,
+                              C.c_uint32, _P]),
     "gnr_profile_enable": (_INT, [_P, _INT]),
     "gnr_profile_collect": (_INT, [_P, C.POINTER(C.c_float), C.POINTER(C.c_int64)]),
     "gnr_measure_l1_bandwidth": (_INT, [_INT, _INT, C.POINTER(C.c_float)]),

@@ -1,0 +1,194 @@
+"""Embedding rows and their gradient (``gnr_embedding_lookup``, ``gnr_embedding_grad``).
+
+``embedding`` looks rows of a table up: the appearance latent of every ray or sample of an ``encode_app`` model
+(``compute_app_latent``, app/models/gridnerf_sequential.py:429-437, does it with one row for all), or any other table's rows.
+``embedding_backward`` is its gradient and, read the other way, the sum of the rows that share an index: samples into rays.
+Both are differentiable, each being the other's gradient.
+
+Indices are int32 or int64, of any shape and strides.  A negative one is a masked place: it looks up zeros and adds nothing.
+One that is not below the number of rows looks up NaN and adds nothing (only the device sees it, so no error is raised).
+Sums are fp32 in an order that only the inputs decide: equal inputs give equal bits.
+"""
+
+from __future__ import annotations
+
+import ctypes as C
+from typing import Optional
+
+import torch
+
+from . import _lib
+from ._lib import check, lib
+
+_TYPES = {torch.float32: _lib.FP32, torch.float16: _lib.FP16, torch.bfloat16: _lib.BF16}
+_INDEX_BITS = {torch.int64: 64, torch.int32: 32}
+
+
+class _on:
+    """Device guard that costs nothing where the tensor's device is the current one."""
+
+    __slots__ = ("guard",)
+
+    def __init__(self, device):
+        self.guard = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
+def _check_values(what: str, t: torch.Tensor, dims: Optional[int] = None) -> int:
+    kind = _TYPES.get(t.dtype)
+    if kind is None:
+        raise TypeError(f"{what} must be float32, float16 or bfloat16, got {t.dtype}")
+    if not t.is_cuda or t.layout is not torch.strided:
+        raise ValueError(f"{what} must be a dense CUDA tensor, got {t.layout} on {t.device}")
+    if dims is not None and t.dim() != dims:
+        raise ValueError(f"{what} must have {dims} dimensions, got {tuple(t.shape)}")
+    return kind
+
+
+def _check_indices(indices: torch.Tensor, device) -> int:
+    bits = _INDEX_BITS.get(indices.dtype)
+    if bits is None:
+        raise TypeError(f"indices must be int64 or int32, got {indices.dtype}")
+    if indices.device != device:
+        raise ValueError(f"indices on {indices.device}, values on {device}")
+    return bits
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """``t [n, d]`` with neighbouring values next to each other and rows that do not overlap."""
+    return t if t.shape[0] == 0 or (t.stride(1) == 1 or t.shape[1] == 1) and (t.stride(0) >= t.shape[1]) else t.contiguous()
+
+
+def _lookup(indices: torch.Tensor, weight: torch.Tensor, scale: float) -> torch.Tensor:
+    kind = _check_values("weight", weight, 2)
+    bits = _check_indices(indices, weight.device)
+    rows, dim = weight.shape
+    if rows == 0 or dim == 0:
+        raise ValueError(f"weight must have a row and a column, got {tuple(weight.shape)}")
+    weight, indices = _rows(weight), indices.contiguous()
+    out = torch.empty((*indices.shape, dim), dtype=weight.dtype, device=weight.device)
+    n = indices.numel()
+    if n:
+        with _on(weight.device):
+            check(lib.gnr_embedding_lookup(weight.data_ptr(), kind, rows, dim, weight.stride(0) if rows > 1 else dim, indices.data_ptr(), bits, n,
+                                           scale, out.data_ptr(), dim, torch.cuda.current_stream(weight.device).cuda_stream),
+                  "gnr_embedding_lookup")
+    return out
+
+
+def _gradient(grad: torch.Tensor, indices: torch.Tensor, num_rows: int, scale: float, padding_idx: Optional[int], out: torch.Tensor,
+              accumulate: bool) -> torch.Tensor:
+    kind, dim, n = _check_values("grad_output", grad), out.shape[1], indices.numel()
+    bits = _check_indices(indices, grad.device)
+    grad, indices = _rows(grad.reshape(n, dim)), indices.contiguous()
+    with _on(grad.device):
+        need = C.c_size_t(0)
+        check(lib.gnr_embedding_grad_workspace_bytes(n, num_rows, dim, C.byref(need)), "gnr_embedding_grad_workspace_bytes")
+        ws = torch.empty(need.value, dtype=torch.uint8, device=grad.device)
+        check(lib.gnr_embedding_grad(grad.data_ptr(), kind, dim, grad.stride(0) if n > 1 else dim, indices.data_ptr(), bits, n, num_rows,
+                                     -1 if padding_idx is None else padding_idx, scale, accumulate, out.data_ptr(), _TYPES[out.dtype],
+                                     out.stride(0) if num_rows > 1 else dim, ws.data_ptr(), need.value,
+                                     torch.cuda.current_stream(grad.device).cuda_stream), "gnr_embedding_grad")
+    return out
+
+
+def _no_capture(what: str):
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError(f"the backward pass of {what} cannot be captured into a CUDA graph: torch would add the gradient to the leaf on the "
+                           "stream of an earlier pass.  Capture embedding() and embedding_backward() themselves, without autograd")
+
+
+class _Embedding(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, indices, weight, scale, padding_idx):
+        ctx.save_for_backward(indices)
+        ctx.args = weight.shape[0], scale, padding_idx, weight.dtype
+        return _lookup(indices, weight, scale)
+
+    @staticmethod
+    def backward(ctx, grad):
+        _no_capture("embedding")
+        rows, scale, padding_idx, dtype = ctx.args
+        return None, embedding_backward(grad, ctx.saved_tensors[0], rows, scale=scale, padding_idx=padding_idx, dtype=dtype), None, None
+
+
+class _EmbeddingBackward(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, grad, indices, num_rows, scale, padding_idx, dtype):
+        ctx.save_for_backward(indices)
+        ctx.args = scale, padding_idx, grad.dtype, grad.shape
+        return _new_gradient(grad, indices, num_rows, scale, padding_idx, dtype)
+
+    @staticmethod
+    def backward(ctx, grad):
+        _no_capture("embedding_backward")
+        scale, padding_idx, dtype, shape = ctx.args
+        indices = ctx.saved_tensors[0]
+        indices = torch.where((indices == (-1 if padding_idx is None else padding_idx)) | (indices >= grad.shape[0]), -1, indices)
+        return embedding(indices, grad, scale=scale).to(dtype).reshape(shape), None, None, None, None, None
+
+
+def _new_gradient(grad, indices, num_rows, scale, padding_idx, dtype):
+    out = torch.empty((num_rows, grad.shape[-1]), dtype=dtype, device=grad.device)
+    return _gradient(grad, indices, num_rows, scale, padding_idx, out, False)
+
+
+def _check_padding(padding_idx: Optional[int], rows: int) -> Optional[int]:
+    if padding_idx is None:
+        return None
+    if not -rows <= padding_idx < rows:
+        raise ValueError(f"padding_idx {padding_idx} is not a row of {rows}")
+    return padding_idx % rows
+
+
+def embedding(indices: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, padding_idx: Optional[int] = None) -> torch.Tensor:
+    """``scale * weight[indices]``: rows of ``weight [rows, dim]`` (float32, float16 or bfloat16), shape ``[*indices.shape, dim]``.
+
+    The product is taken in fp32 and rounded once.  ``padding_idx``: a row that gets no gradient."""
+    _check_values("weight", weight, 2)
+    padding_idx = _check_padding(padding_idx, weight.shape[0])
+    if weight.requires_grad and torch.is_grad_enabled():
+        return _Embedding.apply(indices, weight, float(scale), padding_idx)
+    return _lookup(indices, weight.detach(), float(scale))
+
+
+def embedding_backward(grad_output: torch.Tensor, indices: torch.Tensor, num_rows: int, *, scale: float = 1.0, padding_idx: Optional[int] = None,
+                       dtype: Optional[torch.dtype] = None, out: Optional[torch.Tensor] = None, accumulate: bool = False) -> torch.Tensor:
+    """Gradient of ``embedding`` for its weight: row ``v`` of the result is ``scale`` times the sum of the rows
+    ``grad_output[t]`` with ``indices[t] == v``, and zeros where there is none; ``grad_output [*indices.shape, dim]``.
+
+    ``dtype``: the result's type (that of ``grad_output``).  ``out [num_rows, dim]``: where it is written, or with
+    ``accumulate`` added to; neighbouring values of a row next to each other.  ``padding_idx``: a row that gets nothing."""
+    _check_values("grad_output", grad_output)
+    if grad_output.dim() != indices.dim() + 1 or grad_output.shape[:-1] != indices.shape or grad_output.shape[-1] == 0:
+        raise ValueError(f"grad_output {tuple(grad_output.shape)} does not fit indices {tuple(indices.shape)}")
+    num_rows = int(num_rows)
+    if num_rows < 1:
+        raise ValueError(f"num_rows must be positive, got {num_rows}")
+    padding_idx = _check_padding(padding_idx, num_rows)
+    if out is None:
+        if accumulate:
+            raise ValueError("accumulate needs out")
+        dtype = grad_output.dtype if dtype is None else dtype
+        if dtype not in _TYPES:
+            raise TypeError(f"dtype must be float32, float16 or bfloat16, got {dtype}")
+        if grad_output.requires_grad and torch.is_grad_enabled():
+            return _EmbeddingBackward.apply(grad_output, indices, num_rows, float(scale), padding_idx, dtype)
+        return _new_gradient(grad_output.detach(), indices, num_rows, float(scale), padding_idx, dtype)
+    _check_values("out", out, 2)
+    if dtype is not None and dtype != out.dtype:
+        raise TypeError(f"out is {out.dtype}, dtype {dtype}")
+    if tuple(out.shape) != (num_rows, grad_output.shape[-1]) or out.device != grad_output.device:
+        raise ValueError(f"out {tuple(out.shape)} on {out.device} must be {(num_rows, grad_output.shape[-1])} on {grad_output.device}")
+    if (out.stride(1) != 1 and out.shape[1] > 1) or (num_rows > 1 and out.stride(0) < out.shape[1]):
+        raise ValueError(f"out must have neighbouring values next to each other and rows that do not overlap, got strides {out.stride()}")
+    if torch.is_grad_enabled() and (grad_output.requires_grad or out.requires_grad):
+        raise RuntimeError("embedding_backward writes out in place and is not differentiable then")
+    return _gradient(grad_output, indices, num_rows, float(scale), padding_idx, out, bool(accumulate))

@@ -1,0 +1,225 @@
+"""AdamW over many tensors at once (``gnr_adamw_step``), with optimiser states in 32 or in 8 bits.
+
+The reference trains the planes, lines and network of a field with ``torch.optim.Adam`` over parameter groups; ``AdamW`` takes the
+same groups.  A step is one launch for each parameter type of a group (per 400 tensors), whatever the tensors' sizes; with
+``state_bits=8`` the states take 2 bytes a value instead of 8.
+
+8-bit states: every 256 values of a tensor share two scales; the first moment is ``scale * code``, the second
+``(scale * code) ** 2`` with float8_e4m3fn codes, rounded at random without bias (a hash of seed, step, tensor and place, so a
+step repeats bit for bit).  A gradient that is not finite spoils its own value only.
+
+16-bit parameters can have a copy in fp32 (``masters``): the step updates the copy, the parameter is its rounded image.
+"""
+
+from __future__ import annotations
+
+import ctypes as C
+import operator
+from typing import List, Optional, Sequence, Tuple
+
+import numpy as np
+import torch
+
+from . import _lib
+from ._lib import check, lib
+from .embedding import _TYPES, _on
+
+BLOCK = _lib.ADAMW_BLOCK
+_CODES = torch.float8_e4m3fn
+_WORDS = C.sizeof(_lib.GnrAdamwTensor) // 8  # nine 64-bit words a tensor
+_GRAD, _N = 1, 7
+
+
+def state_blocks(numel: int) -> int:
+    """Scales of a tensor's 8-bit state."""
+    return -(-numel // BLOCK)
+
+
+class AdamWTensors:
+    """Parameters and optimiser states that are stepped together: checked once, then stepped with new gradients.
+
+    ``params``: dense CUDA tensors of one type (float32, float16, bfloat16) on one device; ``exp_avgs`` and ``exp_avg_sqs``: the
+    moments, float32 of the same sizes, or float8_e4m3fn codes with ``exp_avg_scales`` and ``exp_avg_sq_scales`` (float32, one for
+    every 256 values).  ``masters``: float32 copies of 16-bit parameters.  The tensors are updated in place and have to stay
+    where they are: one that was given other memory is refused."""
+
+    def __init__(self, params: Sequence[torch.Tensor], exp_avgs: Sequence[torch.Tensor], exp_avg_sqs: Sequence[torch.Tensor],
+                 exp_avg_scales: Optional[Sequence[torch.Tensor]] = None, exp_avg_sq_scales: Optional[Sequence[torch.Tensor]] = None,
+                 masters: Optional[Sequence[torch.Tensor]] = None):
+        self.params = list(params)
+        if not self.params:
+            raise ValueError("no tensors to step")
+        self.dtype, self.device = self.params[0].dtype, self.params[0].device
+        if self.dtype not in _TYPES:
+            raise TypeError(f"params must be float32, float16 or bfloat16, got {self.dtype}")
+        if self.device.type != "cuda":
+            raise ValueError(f"params must be on a CUDA device, got {self.device}")
+        eight = len(exp_avgs) > 0 and exp_avgs[0].dtype == _CODES
+        self.state_bits = 8 if eight else 32
+        if eight != (exp_avg_scales is not None) or eight != (exp_avg_sq_scales is not None):
+            raise ValueError("exp_avg_scales and exp_avg_sq_scales go with float8_e4m3fn states, and with no others")
+        if masters is not None and self.dtype == torch.float32:
+            raise ValueError("float32 parameters have no masters")
+        state = _CODES if eight else torch.float32
+        sizes = [p.numel() for p in self.params]
+        blocks = [state_blocks(n) for n in sizes]
+        self._tensors = {"params": (self.params, self.dtype, sizes), "exp_avgs": (list(exp_avgs), state, sizes),
+                         "exp_avg_sqs": (list(exp_avg_sqs), state, sizes)}
+        if eight:
+            self._tensors["exp_avg_scales"] = (list(exp_avg_scales), torch.float32, blocks)
+            self._tensors["exp_avg_sq_scales"] = (list(exp_avg_sq_scales), torch.float32, blocks)
+        if masters is not None:
+            self._tensors["masters"] = (list(masters), torch.float32, sizes)
+        self.sizes = sizes
+        self._table = np.zeros((len(sizes), _WORDS), dtype=np.int64)
+        written = set()
+        for column, name in ((0, "params"), (2, "exp_avgs"), (3, "exp_avg_sqs"), (4, "exp_avg_scales"), (5, "exp_avg_sq_scales"), (6, "masters")):
+            if name not in self._tensors:
+                continue
+            tensors, dtype, want = self._tensors[name]
+            if len(tensors) != len(sizes):
+                raise ValueError(f"{len(tensors)} {name} for {len(sizes)} params")
+            for k, (t, n) in enumerate(zip(tensors, want)):
+                if t.dtype != dtype or t.device != self.device or t.numel() != n or t.layout is not torch.strided or not t.is_contiguous():
+                    raise ValueError(f"{name}[{k}] must be {n} contiguous values of {dtype} on {self.device}, got {tuple(t.shape)} of {t.dtype} "
+                                     f"on {t.device}")
+                if n and t.data_ptr() in written:
+                    raise ValueError(f"{name}[{k}] lies in the memory of another tensor of the step")
+                written.add(t.data_ptr())
+                self._table[k, column] = t.data_ptr()
+        self._table[:, _N] = sizes
+        self._table[:, _N + 1] = np.arange(len(sizes))
+        self._places = self._places_now()
+        self.starts = self._places[:len(sizes)]  # addresses of the parameters
+
+    def _places_now(self) -> List[int]:
+        return [p for tensors, _, _ in self._tensors.values() for p in map(torch.Tensor.data_ptr, tensors)]
+
+    def step(self, grads: Sequence[Optional[torch.Tensor]], *, step: int, lr: float, betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
+             weight_decay: float = 1e-2, seed: int = 0):
+        """One step with the gradients ``grads`` (of one type, float32 or 16 bits; None leaves its tensor as it is); ``step``
+        counts from 1.  ``seed``: of the random rounding of 8-bit states."""
+        if len(grads) != len(self.sizes):
+            raise ValueError(f"{len(grads)} gradients for {len(self.sizes)} tensors")
+        if self._places_now() != self._places:
+            raise ValueError("a parameter or state has been given other memory since it was checked")
+        index = self.device.index
+        table = self._table.copy()
+        keep, places, kind = [], [], None
+        for k, (g, n) in enumerate(zip(grads, self.sizes)):
+            if g is None:
+                places.append(0)
+                table[k, _N] = 0
+                continue
+            if g.get_device() != index or g.layout is not torch.strided or g.numel() != n:
+                raise ValueError(f"gradient {k} must be {n} dense values on {self.device}, got {tuple(g.shape)} on {g.device}")
+            if kind is None:
+                kind = g.dtype
+            if g.dtype is not kind or kind not in _TYPES:
+                raise TypeError(f"gradients must be of one type, float32, float16 or bfloat16: got {g.dtype} at {k}, {kind} before")
+            if not g.is_contiguous():
+                g = g.contiguous()
+                keep.append(g)
+            places.append(g.data_ptr())
+        if kind is None:
+            return
+        table[:, _GRAD] = places
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("an AdamW step cannot be captured into a CUDA graph: a replay would repeat this step's count and rates")
+        with _on(self.device):
+            check(lib.gnr_adamw_step(table.ctypes.data, len(places), _TYPES[self.dtype], _TYPES[kind], self.state_bits, step, lr, betas[0], betas[1],
+                                     eps, weight_decay, seed & 0xFFFFFFFF, torch.cuda.current_stream(self.device).cuda_stream), "gnr_adamw_step")
+
+
+def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step: int, lr: float, betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
+               weight_decay: float = 1e-2, exp_avg_scales=None, exp_avg_sq_scales=None, masters=None, seed: int = 0):
+    """One AdamW step over lists of tensors, in place (see ``AdamWTensors``, which checks the lists once for many steps)."""
+    AdamWTensors(params, exp_avgs, exp_avg_sqs, exp_avg_scales, exp_avg_sq_scales, masters).step(
+        grads, step=step, lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, seed=seed)
+
+
+class AdamW(torch.optim.Optimizer):
+    """``torch.optim.AdamW`` over dense CUDA parameters: groups, learning rate schedulers and ``state_dict`` as there.
+
+    ``state_bits``: 32 or 8.  ``master_weights``: 16-bit parameters keep an fp32 copy in the state.  ``seed``: of the random
+    rounding of 8-bit states."""
+
+    def __init__(self, params, lr: float = 1e-3, betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2,
+                 state_bits: int = 32, master_weights: bool = True, seed: int = 0):
+        if state_bits not in (8, 32):
+            raise ValueError(f"state_bits must be 8 or 32, got {state_bits}")
+        if not lr >= 0 or not eps >= 1e-30 or not weight_decay >= 0 or not all(0 <= b < 1 for b in betas):
+            raise ValueError(f"lr {lr}, betas {betas}, eps {eps} (at least 1e-30), weight_decay {weight_decay}")
+        self.state_bits, self.master_weights, self.seed = state_bits, master_weights, seed
+        self._sets: dict = {}  # (group, device, type) -> (parameters, their states by name, AdamWTensors)
+        super().__init__(params, {"lr": lr, "betas": betas, "eps": eps, "weight_decay": weight_decay})
+
+    def add_param_group(self, param_group):
+        super().add_param_group(param_group)
+        self._sets.clear()
+
+    def load_state_dict(self, state_dict):
+        """Restores what ``state_dict`` returned, every state in its own type (torch would give it the parameter's)."""
+        super().load_state_dict(state_dict)
+        self._sets.clear()
+        saved = state_dict["state"]
+        ids = [i for group in state_dict["param_groups"] for i in group["params"]]
+        for i, p in zip(ids, [p for group in self.param_groups for p in group["params"]]):
+            if i in saved:
+                self.state[p] = {k: v.detach().to(p.device, copy=True) if isinstance(v, torch.Tensor) else v for k, v in saved[i].items()}
+
+    def __getstate__(self):
+        return {**super().__getstate__(), "state_bits": self.state_bits, "master_weights": self.master_weights, "seed": self.seed}
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        self._sets = {}
+
+    def _state_of(self, p: torch.Tensor) -> dict:
+        s = self.state[p]
+        if not s:
+            s["step"] = 0
+            kind = _CODES if self.state_bits == 8 else torch.float32
+            for name in ("exp_avg", "exp_avg_sq"):
+                s[name] = torch.zeros(p.shape, dtype=torch.float32 if kind is torch.float32 else torch.uint8, device=p.device)
+                if self.state_bits == 8:
+                    s[name] = s[name].view(kind)
+                    s[name + "_scale"] = torch.zeros(state_blocks(p.numel()), device=p.device)
+            if self.master_weights and p.dtype != torch.float32:
+                s["master"] = p.detach().float()
+        return s
+
+    def _tensors(self, key, params) -> Tuple[list, AdamWTensors]:
+        """States of ``params`` and the checked set of them, made again where a state has been replaced."""
+        states = [self._state_of(p) for p in params]
+        names = [n for n in ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale", "master") if n in states[0]]
+        parts = {n: [s[n] for s in states] for n in names}
+        old = self._sets.get(key)
+        if old is not None and old[2].starts == list(map(torch.Tensor.data_ptr, params)) and old[1].keys() == parts.keys() and all(
+                len(old[1][n]) == len(parts[n]) and all(map(operator.is_, old[1][n], parts[n])) for n in names):
+            return states, old[2]
+        made = AdamWTensors([p.detach() for p in params], parts["exp_avg"], parts["exp_avg_sq"], parts.get("exp_avg_scale"), parts.get("exp_avg_sq_scale"),
+                            parts.get("master"))
+        self._sets[key] = (list(params), parts, made)
+        return states, made
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for number, group in enumerate(self.param_groups):
+            sets: dict = {}
+            for p in group["params"]:
+                if p.grad is not None:
+                    sets.setdefault((number, p.device, p.dtype), []).append(p)
+            for k, (key, params) in enumerate(sets.items()):
+                states, tensors = self._tensors(key, params)
+                for t in sorted({s["step"] for s in states}):  # one, unless a parameter had no gradient in some steps
+                    grads = [p.grad if s["step"] == t else None for p, s in zip(params, states)]
+                    tensors.step(grads, step=int(t) + 1, lr=float(group["lr"]), betas=group["betas"], eps=group["eps"],
+                                 weight_decay=group["weight_decay"], seed=self.seed + 0x3C6EF372 * (2 * number + 1) + k)
+                for s in states:
+                    s["step"] += 1
+        return loss

@@ -1,0 +1,330 @@
+"""AdamW steps against the formula in 64 bits.
+
+With u = 2^-24, each rounded operation of the step is off by at most u of its result:
+  m = b1 m + b1c g      3 u |b1 m| + 3 u |b1c g|  (coefficient, product, sum), rounded up to 4 u each
+  v                     all terms positive: 5 u |v|
+  update = rate * (m / (sqrt(v) / c2 + eps)): the error of m over the same denominator, and 12 u of itself for sqrt, c2, both
+                        quotients, the sum, rate, the product and v's own error
+  p = keep p - update   3 u |keep p| + u |p|"""
+import copy
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+BLOCK = 256
+TOP = 448.0
+
+
+def reference(x, g, m, v, step, lr, betas, eps, decay):
+    """(p, m, v) and how far each may be off, from 64-bit inputs."""
+    b1, b2 = betas
+    m2, v2 = b1 * m + (1 - b1) * g, b2 * v + (1 - b2) * g * g
+    m_tol, v_tol = 4 * U * (b1 * m.abs() + (1 - b1) * g.abs()), 5 * U * v2
+    rate, c2 = lr / (1 - b1 ** step), math.sqrt(1 - b2 ** step)
+    denominator = torch.sqrt(v2) / c2 + eps
+    update = rate * m2 / denominator
+    p = x * (1 - lr * decay) - update
+    return (p, m2, v2), (rate * m_tol / denominator + 12 * U * update.abs() + 3 * U * x.abs() + U * p.abs(), m_tol, v_tol)
+
+
+def tensors(sizes, dtype, grad, seed=0, packed=False):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    starts, at = [], 0
+    for n in sizes:
+        starts.append(at)
+        at += n if packed else -(-n // 64) * 64
+    flat = [torch.randn(at, generator=gen, device="cuda") * s for s in (0.1, 1e-3, 1e-3)] + [torch.rand(at, generator=gen, device="cuda") * 1e-6]
+    flat[1] *= torch.exp(torch.randn(at, generator=gen, device="cuda"))
+    cut = [[f[a:a + n] for n, a in zip(sizes, starts)] for f in flat]
+    p = flat[0].to(dtype)
+    g = flat[1].to(grad)
+    return [p[a:a + n] for n, a in zip(sizes, starts)], [g[a:a + n] for n, a in zip(sizes, starts)], cut[2], cut[3], cut[0]
+
+
+SIZES = [1, 2, 3, 4, 5, 127, 255, 256, 257, 1000, 4095, 4096, 4097, 70001]
+MIXES = [(torch.float32, torch.float32, False), (torch.float32, torch.bfloat16, False), (torch.bfloat16, torch.bfloat16, True),
+         (torch.bfloat16, torch.float32, True), (torch.float16, torch.float16, True), (torch.bfloat16, torch.bfloat16, False),
+         (torch.float16, torch.float32, False)]
+
+
+@pytest.mark.parametrize("dtype,grad,master", MIXES)
+@pytest.mark.parametrize("packed", [False, True])
+def test_step_32bit(dtype, grad, master, packed):
+    from landmark_b200.optim import adamw_step
+
+    for step, betas, decay in ((1, (0.9, 0.999), 0.1), (1000, (0.9, 0.99), 0.0)):
+        p, g, m, v, x = tensors(SIZES, dtype, grad, packed=packed)
+        if not master:
+            x = [t.float() for t in p]
+        want = [reference(a.double(), b.double(), c.double(), d.double(), step, 1e-2, betas, 1e-8, decay) for a, b, c, d in zip(x, g, m, v)]
+        adamw_step(p, g, m, v, step=step, lr=1e-2, betas=betas, weight_decay=decay, masters=x if master else None)
+        for k, ((rp, rm, rv), (tp, tm, tv)) in enumerate(want):
+            assert bool(((m[k].double() - rm).abs() <= tm).all()) and bool(((v[k].double() - rv).abs() <= tv).all()), SIZES[k]
+            if master:
+                assert bool(((x[k].double() - rp).abs() <= tp).all()), SIZES[k]
+                assert torch.equal(p[k], x[k].to(dtype))
+            else:
+                off = 0.0 if dtype == torch.float32 else torch.finfo(dtype).eps / 2 * (rp.abs() + tp) + (2.0 ** -25 if dtype == torch.float16 else 0)
+                assert bool(((p[k].double() - rp).abs() <= tp + off).all()), SIZES[k]
+
+
+# -- 8-bit states: the same separately rounded fp32 operations in torch ------------------------------------------------------
+
+
+def hash32(i, seed):
+    mask = 0xFFFFFFFF
+    x = (i * 0x9E3779B9 + seed) & mask
+    x = x ^ (x >> 16)
+    x = (x * 0x6A09E667) & mask
+    x = x ^ (x >> 15)
+    x = (x * 0xBB67AE85) & mask
+    return x ^ (x >> 16)
+
+
+def encode(x, unit, squared):
+    pad = -x.numel() % BLOCK
+    b, u = torch.nn.functional.pad(x, (0, pad)).view(-1, BLOCK), torch.nn.functional.pad(unit, (0, pad)).view(-1, BLOCK)
+    fine = torch.isfinite(b)
+    top = torch.where(fine, b.abs(), torch.zeros_like(b)).amax(1)
+    top = torch.where(top < 1e-30, torch.zeros_like(top), top)
+    inv = torch.where(top > 0, top.reciprocal() * TOP, torch.zeros_like(top))
+    y = torch.where(fine, b.abs() * inv[:, None], torch.zeros_like(b)).clamp(max=TOP)
+    low = torch.where(y < 2.0 ** -6, torch.floor(y * 512) / 512, (y.view(torch.int32) & ~0xFFFFF).view(torch.float32))
+    step = (y.view(torch.int32) & 0x7F800000).view(torch.float32).clamp(min=2.0 ** -6) / 8
+    up = u * (2 * low + step) * step < (y - low) * (y + low) if squared else u * step < y - low
+    c = torch.where(up, low + step, low)
+    if squared:
+        c = torch.where((y > 0) & (c == 0), torch.full_like(c, 2.0 ** -9), c)
+    c = torch.where(fine, torch.copysign(c, b), torch.full_like(c, float("nan")))
+    return c.view(-1)[:x.numel()], top * (1 / TOP)
+
+
+def random_states(sizes, seed=3):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    codes = [[(torch.randn(n, generator=gen, device="cuda") * 60).clamp(-448, 448).to(torch.float8_e4m3fn) for n in sizes],
+             [(torch.rand(n, generator=gen, device="cuda") * 448).to(torch.float8_e4m3fn) for n in sizes]]
+    scales = [[torch.rand(-(-n // BLOCK), generator=gen, device="cuda") * s for n in sizes] for s in (1e-5, 1e-6)]
+    return codes[0], codes[1], scales[0], scales[1]
+
+
+def bits(t):
+    return t.view(torch.uint8)
+
+
+@pytest.mark.parametrize("dtype,grad,master", MIXES)
+@pytest.mark.parametrize("packed", [False, True])
+def test_step_8bit(dtype, grad, master, packed):
+    from landmark_b200.optim import adamw_step
+
+    step, betas, seed = 37, (0.9, 0.999), 12345
+    p, g, _, _, x = tensors(SIZES, dtype, grad, packed=packed)
+    if not master:
+        x = [t.float() for t in p]
+    m, v, ms, vs = random_states(SIZES)
+    if packed:  # codes that begin at any byte
+        flat = torch.cat([bits(t) for t in m]), torch.cat([bits(t) for t in v])
+        m, v = ([f.view(torch.float8_e4m3fn)[a:a + n] for a, n in zip([sum(SIZES[:k]) for k in range(len(SIZES))], SIZES)] for f in flat)
+    want = []
+    for k, n in enumerate(SIZES):
+        wide = lambda s: s.repeat_interleave(BLOCK)[:n]  # noqa: E731
+        m32, root = m[k].float() * wide(ms[k]), v[k].float() * wide(vs[k])
+        v32, g32 = root * root, g[k].float()
+        f32 = lambda c: torch.tensor(c, dtype=torch.float32, device="cuda")  # noqa: E731
+        ref = reference(x[k].double(), g32.double(), m32.double(), v32.double(), step, 1e-2, betas, 1e-8, 0.1)
+        m32 = f32(betas[0]) * m32 + f32(1 - betas[0]) * g32
+        v32 = f32(betas[1]) * v32 + f32(1 - betas[1]) * g32 * g32
+        h = hash32(torch.arange(n, device="cuda"), hash32(k, hash32(step, seed)))
+        want.append((ref, encode(m32, ((h & 0xFFFF).float() + 0.5) / 65536, False), encode(torch.sqrt(v32), ((h >> 16).float() + 0.5) / 65536, True)))
+    adamw_step(p, g, m, v, step=step, lr=1e-2, betas=betas, weight_decay=0.1, exp_avg_scales=ms, exp_avg_sq_scales=vs,
+               masters=x if master else None, seed=seed)
+    for k, (((rp, _, _), (tp, _, _)), (mc, mscale), (vc, vscale)) in enumerate(want):
+        assert torch.equal(ms[k], mscale) and torch.equal(vs[k], vscale), SIZES[k]
+        assert torch.equal(m[k].float(), mc) and torch.equal(v[k].float(), vc), SIZES[k]
+        if master:
+            assert bool(((x[k].double() - rp).abs() <= tp).all()) and torch.equal(p[k], x[k].to(dtype))
+        else:
+            off = 0.0 if dtype == torch.float32 else torch.finfo(dtype).eps / 2 * (rp.abs() + tp) + (2.0 ** -25 if dtype == torch.float16 else 0)
+            assert bool(((p[k].double() - rp).abs() <= tp + off).all()), SIZES[k]
+
+
+def fresh_8bit(n):
+    return ([torch.zeros(n, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn) for _ in range(2)],
+            [torch.zeros(-(-n // BLOCK), device="cuda") for _ in range(2)])
+
+
+def test_8bit_rounding_keeps_the_mean():
+    """A step that starts from zero states has m = (1 - b1) g and v = (1 - b2) g^2 exactly; over 1024 seeds the mean of what the codes
+    stand for may be off by 6 standard errors of a variable within one code step (standard deviation at most half of it), and by the
+    2^-17 that 16 random bits leave of a step."""
+    from landmark_b200.optim import adamw_step
+
+    n, seeds = 512, 1024
+    g = torch.randn(n, device="cuda") * torch.exp(torch.randn(n, device="cuda"))
+    m_sum, v_sum = torch.zeros(n, dtype=torch.float64, device="cuda"), torch.zeros(n, dtype=torch.float64, device="cuda")
+    for seed in range(seeds):
+        (m, v), (ms, vs) = fresh_8bit(n)
+        adamw_step([torch.zeros(n, device="cuda")], [g], [m], [v], step=1, lr=0.0, exp_avg_scales=[ms], exp_avg_sq_scales=[vs], seed=seed)
+        m_sum += m.double() * ms.double().repeat_interleave(BLOCK)
+        v_sum += (v.double() * vs.double().repeat_interleave(BLOCK)) ** 2
+    allowed = 6 * 0.5 / math.sqrt(seeds) + 2.0 ** -17
+    for total, exact, scale in ((m_sum, 0.1 * g.double(), ms), (v_sum, 1e-3 * g.double() ** 2, vs)):
+        s = scale.double().repeat_interleave(BLOCK)
+        y = exact.abs() / s if total is m_sum else exact.sqrt() / s
+        width = torch.exp2(torch.floor(torch.log2(y.clamp(2.0 ** -6, 447.9)))) / 8  # one code
+        width = width * s if total is m_sum else (2 * y + width) * width * s * s
+        assert bool(((total / seeds - exact).abs() <= allowed * width + 1e-6 * exact.abs()).all())
+
+
+def test_8bit_special_values():
+    from landmark_b200.optim import adamw_step
+
+    n = 3 * BLOCK + 5
+    g = torch.randn(n, device="cuda") * 1e-3
+    g[10], g[BLOCK + 3] = float("nan"), float("inf")
+    g[2 * BLOCK:3 * BLOCK] = 0.0
+    g[3 * BLOCK] = 1e-12  # beside values a million times as large
+    p = torch.randn(n, device="cuda")
+    before = p.clone()
+    (m, v), (ms, vs) = fresh_8bit(n)
+    adamw_step([p], [g], [m], [v], step=1, lr=1e-2, weight_decay=0.0, exp_avg_scales=[ms], exp_avg_sq_scales=[vs])
+    bad = torch.zeros(n, dtype=torch.bool, device="cuda")
+    bad[10] = bad[BLOCK + 3] = True
+    assert torch.equal(p.isfinite(), ~bad) and torch.equal(m.float().isfinite(), ~bad) and torch.equal(v.float().isfinite(), ~bad)
+    assert bool(ms.isfinite().all()) and float(ms[2]) == 0 and float(vs[2]) == 0 and torch.equal(p[2 * BLOCK:3 * BLOCK], before[2 * BLOCK:3 * BLOCK])
+    assert float(v[3 * BLOCK].float()) == 2.0 ** -9  # never 0 where v is not
+    for t in range(2, 30):  # the rest goes on; no value runs away
+        g[10] = g[BLOCK + 3] = 1e-3
+        adamw_step([p], [g], [m], [v], step=t, lr=1e-2, weight_decay=0.0, exp_avg_scales=[ms], exp_avg_sq_scales=[vs], seed=t)
+    assert float((p - before)[~bad].abs().max()) <= 29 * 1e-2 * math.sqrt(10)
+
+
+def test_many_tensors_and_missing_gradients():
+    """More tensors than one launch takes, some without values, some without a gradient."""
+    from landmark_b200.optim import AdamWTensors
+
+    sizes = [(7 * k) % 300 for k in range(1001)]
+    for eight in (False, True):
+        p, g, m, v, _ = tensors(sizes, torch.float32, torch.float32)
+        scales = ()
+        if eight:
+            m, v, *scales = random_states(sizes)
+        grads = [None if k % 5 == 0 else t for k, t in enumerate(g)]
+        before = [[bits(t.contiguous()).clone() for t in ts] for ts in (p, m, v)]
+        one = [[t.clone() for t in ts] for ts in (p, m, v, *scales)]
+        AdamWTensors(p, m, v, *scales).step(grads, step=4, lr=1e-3, seed=9)
+        for k in range(1001):
+            if grads[k] is None:
+                assert all(torch.equal(bits(t[k]), b[k]) for t, b in zip((p, m, v), before))
+        # in several smaller steps: the same (32 bits) whatever the tensors beside them
+        if not eight:
+            for lo in range(0, 1001, 143):
+                cut = slice(lo, lo + 143)
+                AdamWTensors(one[0][cut], one[1][cut], one[2][cut]).step(grads[cut], step=4, lr=1e-3)
+            assert all(torch.equal(a, b) for ts, us in zip((p, m, v), one) for a, b in zip(ts, us))
+
+
+def test_optimiser_follows_the_formula():
+    """Ten steps of the class, groups of different rates, a parameter that sometimes has no gradient, against 64 bits; every step adds at
+    most the errors above, and an error of p is carried on unchanged."""
+    from landmark_b200.optim import AdamW
+
+    torch.manual_seed(0)
+    p = [torch.nn.Parameter(torch.randn(n, device="cuda")) for n in ((5, 7), (300,), ())]
+    opt = AdamW([{"params": p[:2], "lr": 1e-2}, {"params": p[2:], "betas": (0.8, 0.95)}], lr=1e-3, weight_decay=0.1)
+    x, m, v, steps = [t.detach().double() for t in p], [0 * t.detach().double() for t in p], [0 * t.detach().double() for t in p], [0, 0, 0]
+    for t in range(10):
+        opt.zero_grad()
+        for k in range(3):
+            if k == 1 and t % 3 == 2:
+                continue
+            p[k].grad = torch.randn_like(p[k])
+            steps[k] += 1
+            (x[k], m[k], v[k]), _ = reference(x[k], p[k].grad.double(), m[k], v[k], steps[k], 1e-2 if k < 2 else 1e-3,
+                                              (0.9, 0.999) if k < 2 else (0.8, 0.95), 1e-8, 0.1)
+        opt.step()
+    for k in range(3):
+        assert opt.state[p[k]]["step"] == steps[k]
+        assert bool(((p[k].double() - x[k]).abs() <= 10 * 20 * U * (x[k].abs() + 1)).all())
+
+
+@pytest.mark.parametrize("state_bits", [8, 32])
+def test_optimiser_state_survives(state_bits):
+    from landmark_b200.optim import AdamW
+
+    def model():
+        torch.manual_seed(1)
+        return [torch.nn.Parameter(torch.randn(n, device="cuda").to(d)) for n, d in ((500, torch.float32), (300, torch.bfloat16), (77, torch.bfloat16))]
+
+    def run(p, opt, first, last):
+        for t in range(first, last):
+            for k, q in enumerate(p):
+                gen = torch.Generator(device="cuda").manual_seed(100 * t + k)
+                q.grad = torch.randn(q.shape, generator=gen, device="cuda").to(q.dtype)
+            opt.step()
+
+    a = model()
+    opt = AdamW(a, lr=1e-2, state_bits=state_bits, seed=5)
+    run(a, opt, 0, 3)
+    saved = copy.deepcopy(opt.state_dict())
+    middle = [q.detach().clone() for q in a]
+    run(a, opt, 3, 6)
+    b = [torch.nn.Parameter(q) for q in middle]
+    again = AdamW(b, lr=1e-2, state_bits=state_bits, seed=5)
+    again.load_state_dict(saved)
+    s = again.state[b[1]]
+    assert s["master"].dtype == torch.float32 and s["exp_avg"].dtype == (torch.float8_e4m3fn if state_bits == 8 else torch.float32)
+    run(b, again, 3, 6)
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+    assert all(torch.equal(opt.state[x]["exp_avg"].float(), again.state[y]["exp_avg"].float()) for x, y in zip(a, b))
+    # parameters that are given other memory, as by a module's .to(), are followed
+    a[0].data = a[0].data.clone()
+    run(a, opt, 6, 7)
+    run(b, again, 6, 7)
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def test_memory_that_moved_and_captures_are_refused():
+    from landmark_b200.optim import AdamWTensors
+
+    p, g, m, v, _ = tensors([100, 200], torch.float32, torch.float32)
+    t = AdamWTensors(p, m, v)
+    strided = torch.randn(200, device="cuda")[::2]
+    t.step([strided, g[1]], step=1, lr=1e-3)
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="captured"):
+        with torch.cuda.graph(graph):
+            t.step(g, step=2, lr=1e-3)
+    kept = p[0].clone()
+    p[0].data = p[0].data.clone()
+    with pytest.raises(ValueError, match="other memory"):
+        t.step(g, step=2, lr=1e-3)
+    assert torch.equal(p[0], kept)
+    with pytest.raises(ValueError, match="memory of another"):
+        AdamWTensors([p[0], p[0]], [m[0], m[0].clone()], [v[0], v[0].clone()])
+    for bad in ([g[0]], [g[0], g[1][:5]], [g[0], g[1].cpu()]):
+        with pytest.raises(ValueError):
+            AdamWTensors(p, m, v).step(bad, step=1, lr=1e-3)
+    with pytest.raises(TypeError):
+        AdamWTensors(p, m, v).step([g[0], g[1].bfloat16()], step=1, lr=1e-3)
+    with pytest.raises(TypeError):
+        AdamWTensors(p, m, v).step([g[0].double(), g[1].double()], step=1, lr=1e-3)
+    with pytest.raises(RuntimeError, match="step 0"):
+        AdamWTensors(p, m, v).step(g, step=0, lr=1e-3)
+    with pytest.raises(RuntimeError, match="eps"):
+        AdamWTensors(p, m, v).step(g, step=1, lr=1e-3, eps=0.0)
+
+
+def test_offsets_past_32_bits():
+    from landmark_b200.optim import adamw_step
+
+    n = 2 ** 31 + 1000
+    p, g = torch.full((n,), 0.5, dtype=torch.bfloat16, device="cuda"), torch.full((n,), 0.25, dtype=torch.bfloat16, device="cuda")
+    (m, v), (ms, vs) = fresh_8bit(n)
+    adamw_step([p], [g], [m], [v], step=1, lr=0.25, weight_decay=0.0, exp_avg_scales=[ms], exp_avg_sq_scales=[vs])
+    # equal values: every code is the largest one, and the step is the rate
+    assert bool((bits(m) == 0x7E).all()) and bool((bits(v) == 0x7E).all())
+    assert bool((p == 0.25).all())

@@ -1,0 +1,106 @@
+"""Refusals of the training operators: wrong arguments are named before anything reaches a GPU."""
+import ctypes as C
+
+import pytest
+import torch
+
+
+@pytest.fixture(autouse=True)
+def _library(built_library):
+    pass
+
+
+def test_embedding_refuses():
+    from landmark_b200.embedding import embedding, embedding_backward
+
+    idx, w = torch.zeros(3, dtype=torch.long), torch.zeros(5, 4)
+    with pytest.raises(ValueError, match="CUDA"):
+        embedding(idx, w)
+    with pytest.raises(TypeError, match="float64"):
+        embedding(idx, w.double())
+    with pytest.raises(ValueError, match="CUDA"):
+        embedding_backward(torch.zeros(3, 4), idx, 5)
+    with pytest.raises(TypeError, match="int64"):
+        embedding_backward(torch.zeros(3, 4, dtype=torch.int64), idx, 5)
+
+
+def test_c_entries_refuse():
+    from landmark_b200 import _lib
+
+    lib, p = _lib.lib, C.c_void_p(256)
+    n = C.c_size_t(0)
+    assert lib.gnr_embedding_grad_workspace_bytes(1000, 11500, 48, C.byref(n)) == 0 and n.value >= 16000
+    for t, v, d in ((-1, 5, 4), (2 ** 31, 5, 4), (3, 0, 4), (3, 2 ** 31 - 1, 4), (3, 5, 0)):
+        assert lib.gnr_embedding_grad_workspace_bytes(t, v, d, C.byref(n)) < 0
+        assert lib.gnr_embedding_lookup(p, 0, v, d, d, p, 64, t, 1.0, p, d, None) < 0
+    assert lib.gnr_embedding_grad_workspace_bytes(3, 5, 4, None) < 0
+    assert lib.gnr_embedding_lookup(p, 3, 5, 4, 4, p, 64, 3, 1.0, p, 4, None) < 0  # no such type
+    assert lib.gnr_embedding_lookup(p, 0, 5, 4, 4, p, 16, 3, 1.0, p, 4, None) < 0 and b"16 bits" in lib.gnr_last_error()
+    assert lib.gnr_embedding_lookup(p, 0, 5, 4, 3, p, 64, 3, 1.0, p, 4, None) < 0  # rows that overlap
+    assert lib.gnr_embedding_lookup(None, 0, 5, 4, 4, p, 64, 3, 1.0, p, 4, None) < 0
+    assert lib.gnr_embedding_lookup(None, 0, 5, 4, 4, None, 64, 0, 1.0, None, 4, None) == 0  # nothing to do
+    assert lib.gnr_embedding_grad(p, 0, 4, 4, p, 64, 3, 5, -1, 1.0, 0, p, 0, 4, p, 16, None) < 0 and b"workspace" in lib.gnr_last_error()
+    assert lib.gnr_embedding_grad(p, 0, 4, 4, p, 64, 3, 5, -1, 1.0, 0, p, 0, 3, p, 1 << 30, None) < 0
+    assert lib.gnr_embedding_grad(p, 0, 4, 4, p, 64, 3, 5, -1, 1.0, 0, p, 7, 4, p, 1 << 30, None) < 0
+    assert lib.gnr_embedding_grad(p, 0, 4, 4, None, 64, 3, 5, -1, 1.0, 0, p, 0, 4, p, 1 << 30, None) < 0
+    assert lib.gnr_embedding_grad(p, 0, 4, 4, p, 64, 3, 5, -1, 1.0, 0, p, 0, 4, C.c_void_p(264), 1 << 30, None) < 0  # not on 16 bytes
+
+
+def test_adamw_entry_refuses():
+    from landmark_b200 import _lib
+
+    def call(n=10, bits=32, step=1, lr=1e-3, b1=0.9, b2=0.999, eps=1e-8, decay=0.0, ptype=0, gtype=0, **fields):
+        t = (_lib.GnrAdamwTensor * 1)()
+        for k, v in {"param": 256, "grad": 256, "exp_avg": 256, "exp_avg_sq": 256, "n": n, **fields}.items():
+            setattr(t[0], k, v)
+        return _lib.lib.gnr_adamw_step(t, 1, ptype, gtype, bits, step, lr, b1, b2, eps, decay, 0, None)
+
+    for bad in ({"bits": 16}, {"step": 0}, {"lr": -1.0}, {"lr": float("nan")}, {"lr": float("inf")}, {"b1": 1.0}, {"b2": -0.1}, {"eps": 0.0}, {"eps": float("nan")},
+                {"decay": -1.0}, {"ptype": 5}, {"gtype": -1}, {"n": -1}, {"param": None}, {"grad": None}, {"exp_avg": None}, {"exp_avg_sq": None},
+                {"bits": 8}, {"master": 256}):
+        assert call(**bad) < 0, bad
+        assert _lib.lib.gnr_last_error()
+    assert call(n=0) == 0
+    assert _lib.lib.gnr_adamw_step(None, 0, 0, 0, 32, 1, 1e-3, 0.9, 0.999, 1e-8, 0.0, 0, None) == 0
+
+
+def test_adamw_refuses():
+    from landmark_b200.optim import AdamW, AdamWTensors, state_blocks
+
+    x = torch.zeros(4)
+    with pytest.raises(ValueError, match="CUDA"):
+        AdamWTensors([x], [x], [x])
+    with pytest.raises(TypeError, match="float64"):
+        AdamWTensors([x.double()], [x], [x])
+    with pytest.raises(ValueError, match="no tensors"):
+        AdamWTensors([], [], [])
+    for bad in ({"state_bits": 16}, {"lr": -1.0}, {"eps": 0.0}, {"betas": (1.0, 0.9)}, {"weight_decay": -1.0}):
+        with pytest.raises(ValueError):
+            AdamW([torch.nn.Parameter(x)], **bad)
+    assert [state_blocks(n) for n in (0, 1, 256, 257)] == [0, 1, 1, 2]
+    p = torch.nn.Parameter(x)
+    opt = AdamW([p])
+    opt.step()  # nothing has a gradient
+    p.grad = torch.zeros(4)
+    with pytest.raises(ValueError, match="CUDA"):
+        opt.step()
+
+
+def test_random_bits_are_even():
+    """The hash that decides roundings: over neighbouring places and over neighbouring steps every one of its 32 bits is set in half of
+    the cases (6 standard deviations), and so is the exclusive or of neighbours."""
+    def hash32(i, seed):
+        mask = 0xFFFFFFFF
+        x = (i * 0x9E3779B9 + seed) & mask
+        x = x ^ (x >> 16)
+        x = (x * 0x6A09E667) & mask
+        x = x ^ (x >> 15)
+        x = (x * 0xBB67AE85) & mask
+        return x ^ (x >> 16)
+
+    n = 1 << 16
+    i = torch.arange(n, dtype=torch.int64)
+    for h in (hash32(i, 0), hash32(i, hash32(3, hash32(1000, 7))), hash32(77, hash32(2, hash32(i, 5)))):
+        for x in (h, h ^ h.roll(1), h ^ h.roll(256)):
+            for b in range(32):
+                assert abs(int(((x >> b) & 1).sum()) - n / 2) <= 6 * (n / 4) ** 0.5
