@@ -400,10 +400,23 @@ class B200GridNeRF(torch.nn.Module):
         code = int(app_code.item()) if isinstance(app_code, torch.Tensor) else int(app_code)
         if code != self._app_code:
             self._app_code = code
-            with torch.cuda.device(self.device):
-                self._upload_mlp()
-                if self.appearance_lattice:  # (the latent only moves the layer-1 bias, but an MLP upload marks the lattice stale)
-                    check(lib.gnr_build_appearance_lattice(self._handle, 1, _stream()), "gnr_build_appearance_lattice")
+            self.network_changed()
+
+    def network_changed(self):
+        """Give the library the current basis, network and latent of the selected appearance code, after these have been
+        trained (planes and lines: ``commit``, ``reload_field_async``)."""
+        with torch.cuda.device(self.device):
+            self._upload_mlp()
+            if self.appearance_lattice:  # (the latent only moves the layer-1 bias, but an MLP upload marks the lattice stale)
+                check(lib.gnr_build_appearance_lattice(self._handle, 1, _stream()), "gnr_build_appearance_lattice")
+
+    def app_latents(self, codes: torch.Tensor) -> torch.Tensor:
+        """Latents of many appearance codes (one per ray or per sample), ``[*codes.shape, 48]``; differentiable in the table."""
+        if not self.encode_app:
+            raise ValueError("this model has no appearance codes (args.encode_app)")
+        from .embedding import embedding
+
+        return embedding(codes, self.embedding_app.weight)
 
     @torch.no_grad()
     def updateAlphaMask(self, gridSize=(200, 200, 200), increase_alpha_thresh=0):
