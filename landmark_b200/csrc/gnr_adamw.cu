@@ -26,7 +26,8 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kBlock = GNR_ADAMW_BLOCK;
-constexpr int kChunk = 4096;  // values of a thread block: 16 blocks of codes
+constexpr int kChunk = 4096;                       // values of a thread block
+constexpr int kChunk8 = kThreads / 32 * kBlock;    // ... with 8-bit states: a block of codes for each warp
 constexpr float kTop = 448.0f;
 
 struct Tensor {
@@ -38,7 +39,6 @@ struct Tensor {
   float* v_scale;
   float* master;
   int64_t n;
-  uint32_t first;  // thread blocks before this tensor's
   uint32_t seed;
 };
 
@@ -46,16 +46,17 @@ struct Hyper {
   float b1, b1c, b2, b2c;  // betas and 1 - betas
   float keep;              // 1 - lr * weight decay
   float rate;              // lr / (1 - b1^t)
-  float c2;                // sqrt(1 - b2^t)
+  float c2_inv;            // 1 / sqrt(1 - b2^t)
   float eps;
 };
 
 template <int K> struct Table {
   Hyper h;
   int n;
+  uint32_t first[K];  // thread blocks before each tensor's, apart from the rest so that the search stays in a few cache lines
   Tensor t[K];
 };
-constexpr int kSmall = 24, kLarge = 400;  // tensors of a launch: 2 and 32 KB of arguments
+constexpr int kSmall = 24, kLarge = 400;  // tensors of a launch: 2 and 31 KB of arguments
 static_assert(sizeof(Table<kLarge>) <= 32764, "kernel arguments");
 
 __host__ __device__ __forceinline__ uint32_t hash32(uint32_t i, uint32_t seed) {
@@ -68,14 +69,59 @@ __host__ __device__ __forceinline__ uint32_t hash32(uint32_t i, uint32_t seed) {
   return x ^ (x >> 16);
 }
 
+// Two fp32 numbers in one operation of the packed fp32 instructions: each half rounded as the single operation rounds it.
+struct Two {
+  unsigned long long v;
+};
+__device__ __forceinline__ Two two(float x, float y) {
+  Two r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ Two two(float x) { return two(x, x); }
+__device__ __forceinline__ void split(Two a, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(a.v)); }
+__device__ __forceinline__ Two mul2(Two a, Two b) {
+  Two r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ Two add2(Two a, Two b) {
+  Two r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ Two add2_up(Two a, Two b) {
+  Two r;
+  asm("add.rp.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ Two add2_zero(Two a, Two b) {
+  Two r;
+  asm("add.rz.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
+  Two r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+__device__ __forceinline__ Two sub2(Two a, Two b) { return fma2(b, two(-1.0f), a); }
+
 // m and v after the gradient g
 __device__ __forceinline__ void moments(const Hyper& h, float g, float& m, float& v) {
   m = __fadd_rn(__fmul_rn(h.b1, m), __fmul_rn(h.b1c, g));
   v = __fadd_rn(__fmul_rn(h.b2, v), __fmul_rn(__fmul_rn(h.b2c, g), g));
 }
 
+// 1 / x of a normal number, within one unit of the last place
+__device__ __forceinline__ float quick_rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 __device__ __forceinline__ float stepped(const Hyper& h, float x, float m, float root) {
-  return x * h.keep - h.rate * (m / (root / h.c2 + h.eps));
+  return x * h.keep - h.rate * (m * quick_rcp(root * h.c2_inv + h.eps));
 }
 
 // `count` (at most 4) neighbours from `at`, as one access where all four are there and `wide`
@@ -103,14 +149,14 @@ template <typename T> __device__ __forceinline__ void store4(T* at, bool whole, 
 }
 
 // the tensor that a thread block works on
-template <int K> __device__ __forceinline__ const Tensor& find_tensor(const Table<K>& table) {
+template <int K> __device__ __forceinline__ int find_tensor(const Table<K>& table) {
   int lo = 0, hi = table.n - 1;
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
-    if (table.t[mid].first <= blockIdx.x) lo = mid;
+    if (table.first[mid] <= blockIdx.x) lo = mid;
     else hi = mid - 1;
   }
-  return table.t[lo];
+  return lo;
 }
 
 template <typename P, typename G, bool Master> __device__ __forceinline__ bool all_wide(const Tensor& t, int state_align) {
@@ -121,8 +167,9 @@ template <typename P, typename G, bool Master> __device__ __forceinline__ bool a
 template <typename P, typename G, bool Master, int K>
 __global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__ Table<K> table) {
   const Hyper& h = table.h;
-  const Tensor& t = find_tensor(table);
-  const int64_t begin = (int64_t)(blockIdx.x - t.first) * kChunk;
+  const int number = find_tensor(table);
+  const Tensor& t = table.t[number];
+  const int64_t begin = (int64_t)(blockIdx.x - table.first[number]) * kChunk;
   const bool wide = all_wide<P, G, Master>(t, 16);
   float* m_at = static_cast<float*>(t.m);
   float* v_at = static_cast<float*>(t.v);
@@ -158,118 +205,250 @@ __global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__
 
 // ---- 8-bit states ----------------------------------------------------------------------------------------------------
 
-using Fp8 = __nv_fp8_e4m3;
+constexpr uint32_t kNotFinite = 0x7f800000u;  // bits of |x| from here on: infinities and NaN
+constexpr uint32_t kNanCode = 0x7f;
 
-__device__ __forceinline__ void load_codes(const uint8_t* at, bool whole, int count, float (&x)[4]) {
-  uint32_t bits = 0;
-  if (whole) bits = *reinterpret_cast<const uint32_t*>(at);
-  else
-    for (int k = 0; k < count; ++k) bits |= (uint32_t)at[k] << (8 * k);
+// four e4m3 codes as fp32, exactly
+__device__ __forceinline__ void decode4(uint32_t codes, float (&x)[4]) {
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    Fp8 c;
-    c.__x = (uint8_t)(bits >> (8 * k));
-    x[k] = (float)c;
+  for (int k = 0; k < 4; k += 2) {
+    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(codes >> (8 * k)), __NV_E4M3);
+    const float2 y = __half22float2(h);
+    x[k] = y.x;
+    x[k + 1] = y.y;
   }
 }
 
-__device__ __forceinline__ void store_codes(uint8_t* at, bool whole, int count, const float (&x)[4]) {
-  uint32_t bits = 0;
+// `count` (at most 4) neighbours as they lie in memory, zeros behind them
+template <typename T> __device__ __forceinline__ Pack<T, 4> load_raw(const T* at, bool whole, int count) {
+  if (whole) return *reinterpret_cast<const Pack<T, 4>*>(at);
+  Pack<T, 4> y;
 #pragma unroll
-  for (int k = 0; k < 4; ++k) bits |= (uint32_t)Fp8(x[k]).__x << (8 * k);  // exact: x is an e4m3 value or NaN
-  if (whole) *reinterpret_cast<uint32_t*>(at) = bits;
+  for (int k = 0; k < 4; ++k) y.v[k] = k < count ? at[k] : from_float<T>(0.0f);
+  return y;
+}
+
+__device__ __forceinline__ uint32_t load_codes(const uint8_t* at, bool whole, int count) {
+  if (whole) return *reinterpret_cast<const uint32_t*>(at);
+  uint32_t codes = 0;
+  for (int k = 0; k < count; ++k) codes |= (uint32_t)at[k] << (8 * k);
+  return codes;
+}
+
+__device__ __forceinline__ void store_codes(uint8_t* at, bool whole, int count, uint32_t codes) {
+  if (whole) *reinterpret_cast<uint32_t*>(at) = codes;
   else
-    for (int k = 0; k < count; ++k) at[k] = (uint8_t)(bits >> (8 * k));
+    for (int k = 0; k < count; ++k) at[k] = (uint8_t)(codes >> (8 * k));
 }
 
-__device__ __forceinline__ float finite_or_zero(float x) { return isfinite(x) ? x : 0.0f; }
+// Codes by the bits of an fp32 number: its exponent and three mantissa bits, 960 = (127 - 7) << 3 lower, are the e4m3 code of a
+// value from 2^-6 on.  Below, the codes are 2^-9 apart as in the binade above: 2^-6 is added (kShift) and 8 taken off.
+constexpr float kShift = 0.015625f;
 
-// |x| * inv as one of its two neighbouring e4m3 values, unit in (0, 1) deciding which, with x's sign
-template <bool Squared> __device__ __forceinline__ float code_of(float x, float inv, float unit) {
-  if (!isfinite(x)) return __int_as_float(0x7fc00000);
-  const float y = fminf(__fmul_rn(fabsf(x), inv), kTop);
-  const int bits = __float_as_int(y);
-  const float low = y < 0.015625f ? floorf(y * 512.0f) * 0.001953125f : __int_as_float(bits & ~0xfffff);
-  const float step = fmaxf(__int_as_float(bits & 0x7f800000), 0.015625f) * 0.125f;
-  float c;
-  if (Squared) {
-    const bool up = __fmul_rn(__fmul_rn(unit, __fadd_rn(2.0f * low, step)), step) < __fmul_rn(__fsub_rn(y, low), __fadd_rn(y, low));
-    c = up ? low + step : low;
-    if (y > 0.0f && c == 0.0f) c = 0.001953125f;
-  } else {
-    c = __fmul_rn(unit, step) < __fsub_rn(y, low) ? low + step : low;
+// |m| * inv rounded up where a uniform u = (r + 1/2) / 2^16 is below the part of it past the code below: adding 1 - u of a code, less
+// one, to the bits carries into the code in just these cases (u has 17 bits, the part 20; rounded upwards where the shift cuts it).
+__device__ __forceinline__ void codes_of_m(const float (&m)[2], Two inv, const uint32_t (&r32)[2], uint32_t (&code)[2]) {
+  float y[2], shift[2], z[2];
+  split(mul2(two(m[0], m[1]), inv), y[0], y[1]);
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    y[k] = fminf(fabsf(y[k]), kTop);
+    shift[k] = y[k] < kShift ? kShift : 0.0f;
   }
-  return copysignf(c, x);
+  split(add2_up(two(y[0], y[1]), two(shift[0], shift[1])), z[0], z[1]);
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const uint32_t at = (__float_as_uint(z[k]) + ((~r32[k] & 0xffffu) << 4 | 7u)) >> 20;
+    code[k] = (at - (y[k] < kShift ? 968u : 960u)) | (__float_as_uint(m[k]) >> 24 & 0x80u);
+  }
 }
 
-// largest of a warp's non-negative numbers
-__device__ __forceinline__ float warp_top(float x) { return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(x))); }
+// root * inv rounded so that the mean of its square is kept: up where u < (y^2 - low^2) / ((low + step)^2 - low^2)
+__device__ __forceinline__ void codes_of_root(const float (&root)[2], Two inv, const uint32_t (&r32)[2], uint32_t (&code)[2]) {
+  float y[2], shift[2], z[2], a[2], b[2];
+  split(mul2(two(root[0], root[1]), inv), y[0], y[1]);
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    y[k] = fminf(y[k], kTop);
+    shift[k] = y[k] < kShift ? kShift : 0.0f;
+  }
+  const Two yy = two(y[0], y[1]), shifts = two(shift[0], shift[1]);
+  split(add2_zero(yy, shifts), z[0], z[1]);
+  const uint32_t z0 = __float_as_uint(z[0]), z1 = __float_as_uint(z[1]);
+  const Two low = sub2(two(__uint_as_float(z0 & ~0xfffffu), __uint_as_float(z1 & ~0xfffffu)), shifts);
+  const Two step = mul2(two(__uint_as_float(z0 & 0x7f800000u), __uint_as_float(z1 & 0x7f800000u)), two(0.125f));
+  const Two u = add2(two(__uint_as_float(0x3f800040u | (r32[0] >> 16) << 7), __uint_as_float(0x3f800040u | (r32[1] >> 16) << 7)), two(-1.0f));
+  split(mul2(mul2(u, fma2(two(2.0f), low, step)), step), a[0], a[1]);
+  split(mul2(sub2(yy, low), add2(yy, low)), b[0], b[1]);
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const uint32_t at = (__float_as_uint(z[k]) >> 20) - (y[k] < kShift ? 968u : 960u) + (a[k] < b[k] ? 1u : 0u);
+    code[k] = max(at, min(__float_as_uint(root[k]), 1u));  // never 0 where the root is not
+  }
+}
 
-// a warp takes one block of 256 values at a time, a lane the four at 4 * lane and the four 128 behind them
-template <typename P, typename G, bool Master, int K>
-__global__ void __launch_bounds__(kThreads) adamw_8bit_kernel(const __grid_constant__ Table<K> table) {
-  const Hyper& h = table.h;
-  const Tensor& t = find_tensor(table);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const bool wide = all_wide<P, G, Master>(t, 4);
-  uint8_t* m_at = static_cast<uint8_t*>(t.m);
-  uint8_t* v_at = static_cast<uint8_t*>(t.v);
-  constexpr int kEach = kChunk / kBlock / (kThreads / 32);
-  for (int r = 0; r < kEach; ++r) {
-    const int64_t block = (int64_t)(blockIdx.x - t.first) * (kChunk / kBlock) + r * (kThreads / 32) + warp;
-    if (block * kBlock >= t.n) return;
-    const float m_scale = t.m_scale[block], v_scale = t.v_scale[block];
-    float x[2][4], g[2][4], m[2][4], v[2][4];
-    float m_top = 0.0f, v_top = 0.0f;
+// a lane's part of a block of 256 values as it lies in memory: the four values at 4 * lane and the four 128 behind them
+template <typename X, typename G> struct Part {
+  Pack<X, 4> x[2];
+  Pack<G, 4> g[2];
+  uint32_t m[2], v[2];
+  float m_scale, v_scale;
+};
+
+// A thread block's values of a tensor with 8-bit states; all places count from their beginning.
+// 448 / top, 0 for 0: the quick reciprocal and one Newton step (rounded like the exact one but for some in a million)
+__device__ __forceinline__ float scale_up(float top) {
+  if (top > 1e30f) return __fmul_rn(__frcp_rn(top), kTop);
+  const float r = quick_rcp(top);
+  return top > 0.0f ? __fmul_rn(__fmaf_rn(r, __fmaf_rn(-top, r, 1.0f), r), kTop) : 0.0f;
+}
+
+template <typename P, typename G, bool Master> struct Chunk8 {
+  using X = std::conditional_t<Master, float, P>;
+  P* p_at;
+  const G* g_at;
+  uint8_t *m_at, *v_at;
+  float *ms_at, *vs_at, *master_at;
+  int left;        // values there are
+  uint32_t place;  // low half of the first one's place in the tensor
+  uint32_t seed;
+
+  // the part at `at` = 4 * lane past the beginning of a block
+  template <bool Full> __device__ __forceinline__ Part<X, G> fetch(int at) const {
+    Part<X, G> part;
+    const X* x_at = Master ? reinterpret_cast<const X*>(master_at) : reinterpret_cast<const X*>(p_at);
+    part.m_scale = ms_at[at / kBlock];
+    part.v_scale = vs_at[at / kBlock];
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-      const int64_t i = block * kBlock + s * 128 + lane * 4;
-      const int count = (int)max((int64_t)0, min((int64_t)4, t.n - i));
-      const bool whole = wide && count == 4;
-      load4(static_cast<const G*>(t.g) + i, whole, count, g[s]);
-      load_codes(m_at + i, whole, count, m[s]);
-      load_codes(v_at + i, whole, count, v[s]);
-      if constexpr (Master) load4(t.master + i, whole, count, x[s]);
-      else load4(static_cast<const P*>(t.p) + i, whole, count, x[s]);
+      const int i = at + s * 128;
+      const int count = Full ? 4 : min(4, max(0, left - i));
+      part.g[s] = load_raw(g_at + i, Full, count);
+      part.m[s] = load_codes(m_at + i, Full, count);
+      part.v[s] = load_codes(v_at + i, Full, count);
+      part.x[s] = load_raw(x_at + i, Full, count);
+    }
+    return part;
+  }
+
+  template <bool Full> __device__ __forceinline__ void step(const Hyper& h, const Part<X, G>& part, int at) const {
+    float x[2][4], g[2][4], m[2][4], root[2][4];
+    uint32_t m_bits = 0, v_bits = 0;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      decode4(part.m[s], m[s]);
+      decode4(part.v[s], root[s]);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const float root = __fmul_rn(v[s][k], v_scale);
-        m[s][k] = __fmul_rn(m[s][k], m_scale);
-        v[s][k] = __fmul_rn(root, root);
-        moments(h, g[s][k], m[s][k], v[s][k]);
-        v[s][k] = __fsqrt_rn(v[s][k]);
-        x[s][k] = stepped(h, x[s][k], m[s][k], v[s][k]);
-        m_top = fmaxf(m_top, finite_or_zero(fabsf(m[s][k])));
-        v_top = fmaxf(v_top, finite_or_zero(v[s][k]));
+        g[s][k] = to_float(part.g[s].v[k]);
+        x[s][k] = to_float(part.x[s].v[k]);
       }
     }
-    m_top = warp_top(m_top);
-    v_top = warp_top(v_top);
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+#pragma unroll
+      for (int k = 0; k < 4; k += 2) {
+        const Two gg = two(g[s][k], g[s][k + 1]), old = mul2(two(root[s][k], root[s][k + 1]), two(part.v_scale));
+        // (the sums as single additions: a packed one behind packed products is compiled to a fused multiply-add)
+        float old_m[2], new_m[2], old_v[2], new_v[2];
+        split(mul2(two(h.b1), mul2(two(m[s][k], m[s][k + 1]), two(part.m_scale))), old_m[0], old_m[1]);
+        split(mul2(two(h.b1c), gg), new_m[0], new_m[1]);
+        split(mul2(two(h.b2), mul2(old, old)), old_v[0], old_v[1]);
+        split(mul2(mul2(two(h.b2c), gg), gg), new_v[0], new_v[1]);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          m[s][k + j] = __fadd_rn(old_m[j], new_m[j]);
+          root[s][k + j] = __fsqrt_rn(__fadd_rn(old_v[j], new_v[j]));
+        }
+        float d0, d1;
+        split(fma2(two(root[s][k], root[s][k + 1]), two(h.c2_inv), two(h.eps)), d0, d1);
+        const Two q = mul2(two(m[s][k], m[s][k + 1]), two(quick_rcp(d0), quick_rcp(d1)));
+        split(fma2(two(-h.rate), q, mul2(two(x[s][k], x[s][k + 1]), two(h.keep))), x[s][k], x[s][k + 1]);
+        m_bits = max(max(m_bits, __float_as_uint(m[s][k]) & 0x7fffffffu), __float_as_uint(m[s][k + 1]) & 0x7fffffffu);
+        v_bits = max(max(v_bits, __float_as_uint(root[s][k])), __float_as_uint(root[s][k + 1]));
+      }
+      const int i = at + s * 128;
+      const int count = Full ? 4 : min(4, max(0, left - i));
+      if constexpr (Master) store4(master_at + i, Full, count, x[s]);
+      store4(p_at + i, Full, count, x[s]);
+    }
+    m_bits = __reduce_max_sync(0xffffffffu, m_bits);  // non-negative numbers are ordered as their bits are
+    v_bits = __reduce_max_sync(0xffffffffu, v_bits);
+    const bool odd = max(m_bits, v_bits) >= kNotFinite;  // a value that is not finite: the others' scale leaves it out
+    if (odd) {
+      m_bits = v_bits = 0;
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t a = __float_as_uint(m[s][k]) & 0x7fffffffu, b = __float_as_uint(root[s][k]) & 0x7fffffffu;
+          m_bits = max(m_bits, a < kNotFinite ? a : 0u);
+          v_bits = max(v_bits, b < kNotFinite ? b : 0u);
+        }
+      m_bits = __reduce_max_sync(0xffffffffu, m_bits);
+      v_bits = __reduce_max_sync(0xffffffffu, v_bits);
+    }
+    float m_top = __uint_as_float(m_bits), v_top = __uint_as_float(v_bits);
     if (m_top < 1e-30f) m_top = 0.0f;  // 448 / m_top has to be finite
     if (v_top < 1e-30f) v_top = 0.0f;
-    const float m_inv = m_top > 0.0f ? __fmul_rn(__frcp_rn(m_top), kTop) : 0.0f, v_inv = v_top > 0.0f ? __fmul_rn(__frcp_rn(v_top), kTop) : 0.0f;
+    const float m_inv = scale_up(m_top), v_inv = scale_up(v_top);
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-      const int64_t i = block * kBlock + s * 128 + lane * 4;
-      const int count = (int)max((int64_t)0, min((int64_t)4, t.n - i));
-      const bool whole = wide && count == 4;
-      const uint32_t seed = t.seed + (uint32_t)(i >> 32) * 0xBB67AE85u;
+      const int i = at + s * 128;
+      const int count = Full ? 4 : min(4, max(0, left - i));
+      uint32_t m_codes = 0, v_codes = 0;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const uint32_t r32 = hash32((uint32_t)i + k, seed);
-        m[s][k] = code_of<false>(m[s][k], m_inv, ((float)(r32 & 0xffffu) + 0.5f) * (1.0f / 65536.0f));
-        v[s][k] = code_of<true>(v[s][k], v_inv, ((float)(r32 >> 16) + 0.5f) * (1.0f / 65536.0f));
+      for (int k = 0; k < 4; k += 2) {
+        const uint32_t r32[2] = {hash32(place + i + k, seed), hash32(place + i + k + 1, seed)};
+        const float mk[2] = {m[s][k], m[s][k + 1]}, rk[2] = {root[s][k], root[s][k + 1]};
+        uint32_t m_code[2], v_code[2];
+        codes_of_m(mk, two(m_inv), r32, m_code);
+        codes_of_root(rk, two(v_inv), r32, v_code);
+        m_codes |= (m_code[0] | m_code[1] << 8) << (8 * k);
+        v_codes |= (v_code[0] | v_code[1] << 8) << (8 * k);
       }
-      store_codes(m_at + i, whole, count, m[s]);
-      store_codes(v_at + i, whole, count, v[s]);
-      if constexpr (Master) store4(t.master + i, whole, count, x[s]);
-      store4(static_cast<P*>(t.p) + i, whole, count, x[s]);
+      if (odd) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          if ((__float_as_uint(m[s][k]) & 0x7fffffffu) >= kNotFinite) m_codes = (m_codes & ~(0xffu << (8 * k))) | kNanCode << (8 * k);
+          if ((__float_as_uint(root[s][k]) & 0x7fffffffu) >= kNotFinite) v_codes = (v_codes & ~(0xffu << (8 * k))) | kNanCode << (8 * k);
+        }
+      }
+      store_codes(m_at + i, Full, count, m_codes);
+      store_codes(v_at + i, Full, count, v_codes);
     }
-    if (lane == 0) {
-      t.m_scale[block] = __fmul_rn(m_top, 1.0f / kTop);
-      t.v_scale[block] = __fmul_rn(v_top, 1.0f / kTop);
+    if ((threadIdx.x & 31) == 0) {
+      ms_at[at / kBlock] = __fmul_rn(m_top, 1.0f / kTop);
+      vs_at[at / kBlock] = __fmul_rn(v_top, 1.0f / kTop);
     }
   }
+};
+
+// A warp takes one block of 256 values.  Bound by its 89 instructions a value (packed fp32 ones count for two values) and, at 88 % of
+// the copy rate, by HBM: 335M fp32 values 948 us, 5.68 TB/s.  Five thread blocks to an SM hide the loads better than a
+// longer run of blocks with the next one's loads ahead of the work (1058 us at its best length), six spill (1000 us).
+template <typename P, typename G, bool Master, int K>
+__global__ void __launch_bounds__(kThreads, 5) adamw_8bit_kernel(const __grid_constant__ Table<K> table) {
+  const Hyper& h = table.h;
+  const int number = find_tensor(table);
+  const Tensor& t = table.t[number];
+  const int64_t first = (int64_t)(blockIdx.x - table.first[number]) * kChunk8;
+  Chunk8<P, G, Master> c;
+  c.p_at = static_cast<P*>(t.p) + first;
+  c.g_at = static_cast<const G*>(t.g) + first;
+  c.m_at = static_cast<uint8_t*>(t.m) + first;
+  c.v_at = static_cast<uint8_t*>(t.v) + first;
+  c.ms_at = t.m_scale + first / kBlock;
+  c.vs_at = t.v_scale + first / kBlock;
+  c.master_at = Master ? t.master + first : nullptr;
+  c.left = (int)min((int64_t)kChunk8, t.n - first);
+  c.place = (uint32_t)first;
+  c.seed = t.seed + (uint32_t)(first >> 32) * 0xBB67AE85u;
+  const int lane = threadIdx.x & 31;
+  const int at = (threadIdx.x >> 5) * kBlock;
+  if (at >= c.left) return;
+  if (all_wide<P, G, Master>(t, 4) && at + kBlock <= c.left) c.template step<true>(h, c.template fetch<true>(at + lane * 4), at + lane * 4);
+  else c.template step<false>(h, c.template fetch<false>(at + lane * 4), at + lane * 4);
 }
 
 template <int K> int launch_table(const Table<K>& table, uint32_t blocks, int p_type, int g_type, bool master, int bits, cudaStream_t st) {
@@ -292,6 +471,7 @@ template <int K> int launch_table(const Table<K>& table, uint32_t blocks, int p_
 
 template <int K>
 int step_all(const GnrAdamwTensor* tensors, int n, const Hyper& h, int p_type, int g_type, bool master, int bits, uint32_t seed, cudaStream_t st) {
+  const int chunk = bits == 8 ? kChunk8 : kChunk;
   Table<K> table;
   table.h = h;
   int k = 0;
@@ -301,9 +481,10 @@ int step_all(const GnrAdamwTensor* tensors, int n, const Hyper& h, int p_type, i
     for (; k < n && table.n < K; ++k) {
       const GnrAdamwTensor& t = tensors[k];
       if (t.n == 0) continue;
-      const uint64_t need = (uint64_t)(t.n + kChunk - 1) / kChunk;
+      const uint64_t need = (uint64_t)(t.n + chunk - 1) / chunk;
       if (blocks + need > 0x7fffffff) break;
-      table.t[table.n++] = {t.param, t.grad, t.exp_avg, t.exp_avg_sq, t.exp_avg_scale, t.exp_avg_sq_scale, t.master, t.n, (uint32_t)blocks,
+      table.first[table.n] = (uint32_t)blocks;
+      table.t[table.n++] = {t.param, t.grad, t.exp_avg, t.exp_avg_sq, t.exp_avg_scale, t.exp_avg_sq_scale, t.master, t.n,
                             hash32((uint32_t)t.number, seed)};
       blocks += need;
     }
@@ -349,7 +530,7 @@ extern "C" int gnr_adamw_step(const GnrAdamwTensor* tensors_h, int n_tensors, in
   h.b2c = (float)(1.0 - beta2);
   h.keep = (float)(1.0 - lr * weight_decay);
   h.rate = (float)(lr / (1.0 - pow(beta1, (double)step)));
-  h.c2 = (float)sqrt(1.0 - pow(beta2, (double)step));
+  h.c2_inv = (float)(1.0 / sqrt(1.0 - pow(beta2, (double)step)));
   h.eps = (float)eps;
   const uint32_t of_step = hash32((uint32_t)step, seed + (uint32_t)((uint64_t)step >> 32) * 0xBB67AE85u);
   const cudaStream_t st = (cudaStream_t)stream;

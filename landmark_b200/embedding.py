@@ -25,12 +25,12 @@ _INDEX_BITS = {torch.int64: 64, torch.int32: 32}
 
 
 class _on:
-    """Device guard that costs nothing where the tensor's device is the current one."""
+    """Device guard that costs nothing where the device is the current one."""
 
     __slots__ = ("guard",)
 
-    def __init__(self, device):
-        self.guard = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    def __init__(self, index: int):
+        self.guard = None if index == torch.cuda.current_device() else torch.cuda.device(index)
 
     def __enter__(self):
         if self.guard is not None:
@@ -41,61 +41,85 @@ class _on:
             self.guard.__exit__(*exc)
 
 
-def _check_values(what: str, t: torch.Tensor, dims: Optional[int] = None) -> int:
+def _raw_stream(index: int) -> int:
+    return torch.cuda.current_stream(index).cuda_stream
+
+
+# the same without a Stream object in between (2 us a call), where this torch has it
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _raw_stream)
+
+
+def _kind(what: str, t: torch.Tensor) -> int:
     kind = _TYPES.get(t.dtype)
     if kind is None:
         raise TypeError(f"{what} must be float32, float16 or bfloat16, got {t.dtype}")
     if not t.is_cuda or t.layout is not torch.strided:
         raise ValueError(f"{what} must be a dense CUDA tensor, got {t.layout} on {t.device}")
-    if dims is not None and t.dim() != dims:
-        raise ValueError(f"{what} must have {dims} dimensions, got {tuple(t.shape)}")
     return kind
 
 
-def _check_indices(indices: torch.Tensor, device) -> int:
+def _index_bits(indices: torch.Tensor, index: int) -> int:
     bits = _INDEX_BITS.get(indices.dtype)
     if bits is None:
         raise TypeError(f"indices must be int64 or int32, got {indices.dtype}")
-    if indices.device != device:
-        raise ValueError(f"indices on {indices.device}, values on {device}")
+    if indices.get_device() != index:
+        raise ValueError(f"indices on {indices.device}, values on cuda:{index}")
     return bits
 
 
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    """``t [n, d]`` with neighbouring values next to each other and rows that do not overlap."""
-    return t if t.shape[0] == 0 or (t.stride(1) == 1 or t.shape[1] == 1) and (t.stride(0) >= t.shape[1]) else t.contiguous()
+def _rows(t: torch.Tensor):
+    """``t [n, d]`` with neighbouring values next to each other and rows that do not overlap, and the rows' distance."""
+    if t.is_contiguous():
+        return t, t.shape[1]
+    if t.shape[0] > 1 and (t.stride(1) == 1 or t.shape[1] == 1) and t.stride(0) >= t.shape[1]:
+        return t, t.stride(0)
+    return t.contiguous(), t.shape[1]
 
 
 def _lookup(indices: torch.Tensor, weight: torch.Tensor, scale: float) -> torch.Tensor:
-    kind = _check_values("weight", weight, 2)
-    bits = _check_indices(indices, weight.device)
+    kind, device = _kind("weight", weight), weight.get_device()
+    bits = _index_bits(indices, device)
+    if weight.dim() != 2 or weight.numel() == 0:
+        raise ValueError(f"weight must be [rows, dim] with a value at least, got {tuple(weight.shape)}")
     rows, dim = weight.shape
-    if rows == 0 or dim == 0:
-        raise ValueError(f"weight must have a row and a column, got {tuple(weight.shape)}")
-    weight, indices = _rows(weight), indices.contiguous()
-    out = torch.empty((*indices.shape, dim), dtype=weight.dtype, device=weight.device)
+    weight, stride = _rows(weight)
     n = indices.numel()
+    out = weight.new_empty((*indices.shape, dim))
     if n:
-        with _on(weight.device):
-            check(lib.gnr_embedding_lookup(weight.data_ptr(), kind, rows, dim, weight.stride(0) if rows > 1 else dim, indices.data_ptr(), bits, n,
-                                           scale, out.data_ptr(), dim, torch.cuda.current_stream(weight.device).cuda_stream),
-                  "gnr_embedding_lookup")
+        indices = indices.contiguous()
+        with _on(device):
+            check(lib.gnr_embedding_lookup(weight.data_ptr(), kind, rows, dim, stride, indices.data_ptr(), bits, n, scale, out.data_ptr(), dim,
+                                           _raw_stream(device)), "gnr_embedding_lookup")
     return out
 
 
-def _gradient(grad: torch.Tensor, indices: torch.Tensor, num_rows: int, scale: float, padding_idx: Optional[int], out: torch.Tensor,
+_workspace_bytes: dict = {}  # sizes of a call -> bytes the library asks for
+
+
+def _workspace_need(n: int, rows: int, dim: int) -> int:
+    need = _workspace_bytes.get((n, rows, dim))
+    if need is None:
+        size = C.c_size_t(0)
+        check(lib.gnr_embedding_grad_workspace_bytes(n, rows, dim, C.byref(size)), "gnr_embedding_grad_workspace_bytes")
+        if len(_workspace_bytes) > 256:
+            _workspace_bytes.clear()
+        need = _workspace_bytes[n, rows, dim] = size.value
+    return need
+
+
+def _gradient(grad: torch.Tensor, indices: torch.Tensor, scale: float, padding_idx: Optional[int], out: torch.Tensor,
               accumulate: bool) -> torch.Tensor:
-    kind, dim, n = _check_values("grad_output", grad), out.shape[1], indices.numel()
-    bits = _check_indices(indices, grad.device)
-    grad, indices = _rows(grad.reshape(n, dim)), indices.contiguous()
-    with _on(grad.device):
-        need = C.c_size_t(0)
-        check(lib.gnr_embedding_grad_workspace_bytes(n, num_rows, dim, C.byref(need)), "gnr_embedding_grad_workspace_bytes")
-        ws = torch.empty(need.value, dtype=torch.uint8, device=grad.device)
-        check(lib.gnr_embedding_grad(grad.data_ptr(), kind, dim, grad.stride(0) if n > 1 else dim, indices.data_ptr(), bits, n, num_rows,
+    kind, device, n = _kind("grad_output", grad), grad.get_device(), indices.numel()
+    bits = _index_bits(indices, device)
+    rows, dim = out.shape
+    grad, stride = _rows(grad if grad.dim() == 2 else grad.reshape(n, dim))
+    indices = indices.contiguous()
+    with _on(device):
+        need = _workspace_need(n, rows, dim)
+        ws = torch.empty(need, dtype=torch.uint8, device=grad.device)
+        check(lib.gnr_embedding_grad(grad.data_ptr(), kind, dim, stride, indices.data_ptr(), bits, n, rows,
                                      -1 if padding_idx is None else padding_idx, scale, accumulate, out.data_ptr(), _TYPES[out.dtype],
-                                     out.stride(0) if num_rows > 1 else dim, ws.data_ptr(), need.value,
-                                     torch.cuda.current_stream(grad.device).cuda_stream), "gnr_embedding_grad")
+                                     out.stride(0) if rows > 1 else dim, ws.data_ptr(), need, _raw_stream(device)), "gnr_embedding_grad")
     return out
 
 
@@ -136,13 +160,10 @@ class _EmbeddingBackward(torch.autograd.Function):
 
 
 def _new_gradient(grad, indices, num_rows, scale, padding_idx, dtype):
-    out = torch.empty((num_rows, grad.shape[-1]), dtype=dtype, device=grad.device)
-    return _gradient(grad, indices, num_rows, scale, padding_idx, out, False)
+    return _gradient(grad, indices, scale, padding_idx, torch.empty((num_rows, grad.shape[-1]), dtype=dtype, device=grad.device), False)
 
 
-def _check_padding(padding_idx: Optional[int], rows: int) -> Optional[int]:
-    if padding_idx is None:
-        return None
+def _check_padding(padding_idx: int, rows: int) -> int:
     if not -rows <= padding_idx < rows:
         raise ValueError(f"padding_idx {padding_idx} is not a row of {rows}")
     return padding_idx % rows
@@ -152,11 +173,11 @@ def embedding(indices: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, p
     """``scale * weight[indices]``: rows of ``weight [rows, dim]`` (float32, float16 or bfloat16), shape ``[*indices.shape, dim]``.
 
     The product is taken in fp32 and rounded once.  ``padding_idx``: a row that gets no gradient."""
-    _check_values("weight", weight, 2)
-    padding_idx = _check_padding(padding_idx, weight.shape[0])
+    if padding_idx is not None:
+        padding_idx = _check_padding(padding_idx, weight.shape[0])
     if weight.requires_grad and torch.is_grad_enabled():
         return _Embedding.apply(indices, weight, float(scale), padding_idx)
-    return _lookup(indices, weight.detach(), float(scale))
+    return _lookup(indices, weight, float(scale))
 
 
 def embedding_backward(grad_output: torch.Tensor, indices: torch.Tensor, num_rows: int, *, scale: float = 1.0, padding_idx: Optional[int] = None,
@@ -166,13 +187,14 @@ def embedding_backward(grad_output: torch.Tensor, indices: torch.Tensor, num_row
 
     ``dtype``: the result's type (that of ``grad_output``).  ``out [num_rows, dim]``: where it is written, or with
     ``accumulate`` added to; neighbouring values of a row next to each other.  ``padding_idx``: a row that gets nothing."""
-    _check_values("grad_output", grad_output)
+    _kind("grad_output", grad_output)
     if grad_output.dim() != indices.dim() + 1 or grad_output.shape[:-1] != indices.shape or grad_output.shape[-1] == 0:
         raise ValueError(f"grad_output {tuple(grad_output.shape)} does not fit indices {tuple(indices.shape)}")
     num_rows = int(num_rows)
     if num_rows < 1:
         raise ValueError(f"num_rows must be positive, got {num_rows}")
-    padding_idx = _check_padding(padding_idx, num_rows)
+    if padding_idx is not None:
+        padding_idx = _check_padding(padding_idx, num_rows)
     if out is None:
         if accumulate:
             raise ValueError("accumulate needs out")
@@ -181,8 +203,8 @@ def embedding_backward(grad_output: torch.Tensor, indices: torch.Tensor, num_row
             raise TypeError(f"dtype must be float32, float16 or bfloat16, got {dtype}")
         if grad_output.requires_grad and torch.is_grad_enabled():
             return _EmbeddingBackward.apply(grad_output, indices, num_rows, float(scale), padding_idx, dtype)
-        return _new_gradient(grad_output.detach(), indices, num_rows, float(scale), padding_idx, dtype)
-    _check_values("out", out, 2)
+        return _new_gradient(grad_output, indices, num_rows, float(scale), padding_idx, dtype)
+    _kind("out", out)
     if dtype is not None and dtype != out.dtype:
         raise TypeError(f"out is {out.dtype}, dtype {dtype}")
     if tuple(out.shape) != (num_rows, grad_output.shape[-1]) or out.device != grad_output.device:
@@ -191,4 +213,4 @@ def embedding_backward(grad_output: torch.Tensor, indices: torch.Tensor, num_row
         raise ValueError(f"out must have neighbouring values next to each other and rows that do not overlap, got strides {out.stride()}")
     if torch.is_grad_enabled() and (grad_output.requires_grad or out.requires_grad):
         raise RuntimeError("embedding_backward writes out in place and is not differentiable then")
-    return _gradient(grad_output, indices, num_rows, float(scale), padding_idx, out, bool(accumulate))
+    return _gradient(grad_output, indices, float(scale), padding_idx, out, bool(accumulate))

@@ -22,12 +22,13 @@ import torch
 
 from . import _lib
 from ._lib import check, lib
-from .embedding import _TYPES, _on
+from .embedding import _TYPES, _on, _raw_stream
 
 BLOCK = _lib.ADAMW_BLOCK
 _CODES = torch.float8_e4m3fn
 _WORDS = C.sizeof(_lib.GnrAdamwTensor) // 8  # nine 64-bit words a tensor
 _GRAD, _N = 1, 7
+_address, _numel, _get_device, _is_contiguous = torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.get_device, torch.Tensor.is_contiguous
 
 
 def state_blocks(numel: int) -> int:
@@ -40,8 +41,8 @@ class AdamWTensors:
 
     ``params``: dense CUDA tensors of one type (float32, float16, bfloat16) on one device; ``exp_avgs`` and ``exp_avg_sqs``: the
     moments, float32 of the same sizes, or float8_e4m3fn codes with ``exp_avg_scales`` and ``exp_avg_sq_scales`` (float32, one for
-    every 256 values).  ``masters``: float32 copies of 16-bit parameters.  The tensors are updated in place and have to stay
-    where they are: one that was given other memory is refused."""
+    every 256 values).  ``masters``: float32 copies of 16-bit parameters.  The tensors are updated in place where they
+    were when this was made; a step with a parameter that was given other memory since is refused."""
 
     def __init__(self, params: Sequence[torch.Tensor], exp_avgs: Sequence[torch.Tensor], exp_avg_sqs: Sequence[torch.Tensor],
                  exp_avg_scales: Optional[Sequence[torch.Tensor]] = None, exp_avg_sq_scales: Optional[Sequence[torch.Tensor]] = None,
@@ -89,11 +90,9 @@ class AdamWTensors:
                 self._table[k, column] = t.data_ptr()
         self._table[:, _N] = sizes
         self._table[:, _N + 1] = np.arange(len(sizes))
-        self._places = self._places_now()
-        self.starts = self._places[:len(sizes)]  # addresses of the parameters
-
-    def _places_now(self) -> List[int]:
-        return [p for tensors, _, _ in self._tensors.values() for p in map(torch.Tensor.data_ptr, tensors)]
+        self.starts = self._table[:, 0].tolist()  # addresses of the parameters
+        # the memory that the table names stays, whatever becomes of the tensors
+        self._kept = [t.detach() for tensors, _, _ in self._tensors.values() for t in tensors]
 
     def step(self, grads: Sequence[Optional[torch.Tensor]], *, step: int, lr: float, betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
              weight_decay: float = 1e-2, seed: int = 0):
@@ -101,34 +100,47 @@ class AdamWTensors:
         counts from 1.  ``seed``: of the random rounding of 8-bit states."""
         if len(grads) != len(self.sizes):
             raise ValueError(f"{len(grads)} gradients for {len(self.sizes)} tensors")
-        if self._places_now() != self._places:
-            raise ValueError("a parameter or state has been given other memory since it was checked")
+        if list(map(_address, self.params)) != self.starts:
+            raise ValueError("a parameter has been given other memory since it was checked")
         index = self.device.index
         table = self._table.copy()
-        keep, places, kind = [], [], None
+        try:  # all there and as they should be
+            kinds = {g.dtype for g in grads}
+            plain = (list(map(_numel, grads)) == self.sizes and set(map(_get_device, grads)) == {index} and len(kinds) == 1
+                     and all(map(_is_contiguous, grads)) and kinds <= _TYPES.keys())
+            if plain:
+                table[:, _GRAD] = list(map(_address, grads))
+        except (AttributeError, TypeError, RuntimeError):
+            plain = False
+        if plain:
+            (kind,) = kinds
+        else:
+            grads, kind = self._grads(grads, table)
+            if kind is None:
+                return
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("an AdamW step cannot be captured into a CUDA graph: a replay would repeat this step's count and rates")
+        with _on(index):
+            check(lib.gnr_adamw_step(table.ctypes.data, len(table), _TYPES[self.dtype], _TYPES[kind], self.state_bits, step, lr, betas[0], betas[1],
+                                     eps, weight_decay, seed & 0xFFFFFFFF, _raw_stream(index)), "gnr_adamw_step")
+
+    def _grads(self, grads, table):
+        """Gradients one by one: some missing, not contiguous or wrong.  Returns what has to stay until the launch, and their type."""
+        kept, kind = [], None
         for k, (g, n) in enumerate(zip(grads, self.sizes)):
             if g is None:
-                places.append(0)
                 table[k, _N] = 0
                 continue
-            if g.get_device() != index or g.layout is not torch.strided or g.numel() != n:
+            if g.get_device() != self.device.index or g.layout is not torch.strided or g.numel() != n:
                 raise ValueError(f"gradient {k} must be {n} dense values on {self.device}, got {tuple(g.shape)} on {g.device}")
             if kind is None:
                 kind = g.dtype
             if g.dtype is not kind or kind not in _TYPES:
                 raise TypeError(f"gradients must be of one type, float32, float16 or bfloat16: got {g.dtype} at {k}, {kind} before")
-            if not g.is_contiguous():
-                g = g.contiguous()
-                keep.append(g)
-            places.append(g.data_ptr())
-        if kind is None:
-            return
-        table[:, _GRAD] = places
-        if torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("an AdamW step cannot be captured into a CUDA graph: a replay would repeat this step's count and rates")
-        with _on(self.device):
-            check(lib.gnr_adamw_step(table.ctypes.data, len(places), _TYPES[self.dtype], _TYPES[kind], self.state_bits, step, lr, betas[0], betas[1],
-                                     eps, weight_decay, seed & 0xFFFFFFFF, torch.cuda.current_stream(self.device).cuda_stream), "gnr_adamw_step")
+            g = g.contiguous()
+            kept.append(g)
+            table[k, _GRAD] = g.data_ptr()
+        return kept, kind
 
 
 def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step: int, lr: float, betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
@@ -195,7 +207,7 @@ class AdamW(torch.optim.Optimizer):
         names = [n for n in ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale", "master") if n in states[0]]
         parts = {n: [s[n] for s in states] for n in names}
         old = self._sets.get(key)
-        if old is not None and old[2].starts == list(map(torch.Tensor.data_ptr, params)) and old[1].keys() == parts.keys() and all(
+        if old is not None and old[2].starts == list(map(_address, params)) and old[1].keys() == parts.keys() and all(
                 len(old[1][n]) == len(parts[n]) and all(map(operator.is_, old[1][n], parts[n])) for n in names):
             return states, old[2]
         made = AdamWTensors([p.detach() for p in params], parts["exp_avg"], parts["exp_avg_sq"], parts.get("exp_avg_scale"), parts.get("exp_avg_sq_scale"),

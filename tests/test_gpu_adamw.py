@@ -3,8 +3,9 @@
 With u = 2^-24, each rounded operation of the step is off by at most u of its result:
   m = b1 m + b1c g      3 u |b1 m| + 3 u |b1c g|  (coefficient, product, sum), rounded up to 4 u each
   v                     all terms positive: 5 u |v|
-  update = rate * (m / (sqrt(v) / c2 + eps)): the error of m over the same denominator, and 12 u of itself for sqrt, c2, both
-                        quotients, the sum, rate, the product and v's own error
+  update = rate * (m / (sqrt(v) / c2 + eps)): the error of m over the same denominator, and of itself 2.5 u for v's error under
+                        the root, 1 for the root, 2 for 1 / c2 and its product, 1 for the sum, 2 for a reciprocal within one unit
+                        of the last place, 1 for its product with m, 2 for rate and its product: 11.5 u, rounded up to 12
   p = keep p - update   3 u |keep p| + u |p|"""
 import copy
 import math
