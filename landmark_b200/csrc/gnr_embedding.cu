@@ -6,9 +6,16 @@
 // Gradient: out[v] = round(scale * sum over t with i_t = v of grad[t]), every row of the table written.  The tokens are
 // sorted by index (a stable radix sort of (index, token) pairs), then summed in the sorted order, fp32, without atomics on
 // floats: the same inputs give the same bits.  The sum is split evenly over the sorted tokens, not over the rows, so one
-// row that all tokens name costs no more than many short ones: a worker takes `L` consecutive sorted tokens, writes the rows
-// that begin and end inside its share, and leaves the pieces of the others to be joined, first in its block, then
-// (join kernel) between blocks, always in the order of the tokens.
+// row that all tokens name costs no more than many short ones: a worker takes `share` consecutive sorted tokens, writes the
+// rows that begin and end inside its share, and leaves the pieces of the others to be joined, first in its block, then
+// (join kernel) between blocks, always in the order of the tokens.  Rows that no token names are filled with zeros by further
+// blocks of the same launch.
+//
+// Three ways to sort, by the number of tokens: up to 1024, every block that sums sorts all of them itself (one launch for
+// the whole gradient where one block can sum them); up to 65536, a cluster of eight blocks sorts in its shared memory; above, tiles of
+// 4096 tokens are counted, scanned and scattered digit by digit.
+#include <cooperative_groups.h>
+
 #include <algorithm>
 
 #include "gnr_internal.cuh"
@@ -20,83 +27,141 @@ constexpr int kThreads = 256;
 
 // ---- lookup --------------------------------------------------------------------------------------------------------
 
-// One thread per N values of the output; `per_row` such pieces make a row.
+constexpr int kPieces = 4;  // pieces of a thread
+
+// A piece is N neighbouring values of the output; `per_row` of them make a row.  A thread has kPieces of them, kThreads apart
+// (hop_rows rows and hop_pieces pieces from one to the next), all of them in flight at once.
 template <typename T, typename I, int N>
 __global__ void __launch_bounds__(kThreads)
-embedding_lookup_kernel(const T* __restrict__ table, int64_t rows, int64_t table_stride, const I* __restrict__ index, int64_t n_pieces,
-                        uint32_t per_row, float scale, T* __restrict__ out, int64_t out_stride) {
-  const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  if (i >= n_pieces) return;
-  const int64_t t = i / per_row;
-  const int64_t c = (i - t * per_row) * N;
-  const int64_t row = (int64_t)index[t];
-  Pack<T, N> x;
-  if (row >= 0 && row < rows) {
-    x = *reinterpret_cast<const Pack<T, N>*>(table + row * table_stride + c);
+embedding_lookup_kernel(const T* __restrict__ table, int64_t rows, int64_t table_stride, const I* __restrict__ index, int64_t n, uint32_t per_row,
+                        uint32_t hop_rows, uint32_t hop_pieces, float scale, T* __restrict__ out, int64_t out_stride) {
+  const uint64_t first = (uint64_t)blockIdx.x * (kThreads * kPieces);
+  int64_t t = (int64_t)(first / per_row);
+  uint32_t c = (uint32_t)(first - (uint64_t)t * per_row) + threadIdx.x;
+  t += c / per_row;
+  c %= per_row;
+  int64_t row[kPieces];
+  T* to[kPieces];
+  Raw<T, N> x[kPieces];
 #pragma unroll
-    for (int k = 0; k < N; ++k) x.v[k] = from_float<T>(to_float(x.v[k]) * scale);
-  } else {  // a masked place gives zeros, an index past the table NaN
-    const T fill = from_float<T>(row < 0 ? 0.0f : __int_as_float(0x7fc00000));
-#pragma unroll
-    for (int k = 0; k < N; ++k) x.v[k] = fill;
+  for (int k = 0; k < kPieces; ++k) {
+    row[k] = t < n ? (int64_t)index[t] : -1;
+    to[k] = t < n ? out + t * out_stride + (int64_t)c * N : nullptr;
+    if (row[k] >= 0 && row[k] < rows) {
+      const T* from = table + row[k] * table_stride + (int64_t)c * N;
+      if constexpr (sizeof(T) * N == 32) load32(x[k], from);
+      else x[k].load(from);
+    }
+    t += hop_rows;
+    c += hop_pieces;
+    if (c >= per_row) {
+      c -= per_row;
+      ++t;
+    }
   }
-  *reinterpret_cast<Pack<T, N>*>(out + t * out_stride + c) = x;
+#pragma unroll
+  for (int k = 0; k < kPieces; ++k) {
+    if (!to[k]) continue;
+    Pack<T, N> y;
+    if (row[k] >= 0 && row[k] < rows) {
+#pragma unroll
+      for (int j = 0; j < N; ++j) y.v[j] = from_float<T>(x[k].get(j) * scale);
+    } else {  // a masked place gives zeros, an index past the table NaN
+      const T fill = from_float<T>(row[k] < 0 ? 0.0f : __int_as_float(0x7fc00000));
+#pragma unroll
+      for (int j = 0; j < N; ++j) y.v[j] = fill;
+    }
+    if constexpr (sizeof(T) * N == 32) store32(to[k], y);
+    else *reinterpret_cast<Pack<T, N>*>(to[k]) = y;
+  }
 }
 
 // ---- sort ----------------------------------------------------------------------------------------------------------
 
-constexpr int kSortThreads = 512;
-constexpr int kSortWarps = kSortThreads / 32;
-constexpr int kItems = 8;                      // tokens of a thread
-constexpr int kTile = kSortThreads * kItems;   // tokens of a block
-constexpr int kMaxBits = 9;                    // bits of a digit
+constexpr int kMaxBits = 9;  // bits of a digit
 constexpr int kMaxRadix = 1 << kMaxBits;
+constexpr uint32_t kNoKey = 0xffffffffu;
 
-struct SortShared {
-  uint16_t warp_count[kSortWarps][kMaxRadix];  // tokens of a digit in a warp's share, then before it in the block
-  uint32_t base[kMaxRadix];
-  uint32_t scan[kSortWarps];
+// Tokens to sort: their indices as the caller gave them, 32 or 64 bits wide.
+struct Tokens {
+  const void* index;
+  int wide;
+  int64_t n, rows, padding;
+  // a token's key: its row, or `rows` for what the gradient leaves out (masked, past the table, the padding row)
+  __device__ __forceinline__ uint32_t key_of(int64_t i) const { return i < 0 || i >= rows || i == padding ? (uint32_t)rows : (uint32_t)i; }
+  __device__ __forceinline__ uint32_t key(int64_t t) const {
+    return key_of(wide ? static_cast<const int64_t*>(index)[t] : static_cast<const int32_t*>(index)[t]);
+  }
+  // keys of several tokens (0 for those past the last), all loads in flight at once
+  template <int Items, typename At> __device__ __forceinline__ void keys(At at, uint32_t (&key)[Items]) const {
+    if (wide) {
+      int64_t i[Items];
+#pragma unroll
+      for (int j = 0; j < Items; ++j) i[j] = at(j) < n ? static_cast<const int64_t*>(index)[at(j)] : 0;
+#pragma unroll
+      for (int j = 0; j < Items; ++j) key[j] = key_of(i[j]);
+    } else {
+      int32_t i[Items];
+#pragma unroll
+      for (int j = 0; j < Items; ++j) i[j] = at(j) < n ? static_cast<const int32_t*>(index)[at(j)] : 0;
+#pragma unroll
+      for (int j = 0; j < Items; ++j) key[j] = key_of(i[j]);
+    }
+  }
 };
 
-// A token's key: its row, or `rows` for what the gradient leaves out (masked, past the table, the padding row).
-template <typename I> __device__ __forceinline__ uint32_t token_key(I index, int64_t rows, int64_t padding) {
-  const int64_t i = (int64_t)index;
-  return i < 0 || i >= rows || i == padding ? (uint32_t)rows : (uint32_t)i;
-}
+template <int Warps> struct Counts {
+  uint16_t of_warp[Warps][kMaxRadix];  // tokens of a digit in a warp's share, then in the shares before it
+  uint32_t base[kMaxRadix];
+  uint32_t scan[32];
+};
 
 // place of a thread's j-th token in its block's tile: every warp has a run of neighbours
-__device__ __forceinline__ int tile_place(int j) { return (threadIdx.x >> 5) * (32 * kItems) + j * 32 + (threadIdx.x & 31); }
+template <int Items> __device__ __forceinline__ int tile_place(int j) {
+  return (threadIdx.x >> 5) * (32 * Items) + j * 32 + (threadIdx.x & 31);
+}
 
-// Ranks of a tile's tokens among the tokens of the same digit, in the tile's order.  digit < 0: no token.
-// Afterwards warp_count[w][d] holds the tokens of digit d in the warps before w, and the return value of thread d < radix is
-// the number of them in the tile.
-__device__ __forceinline__ uint32_t rank_tile(SortShared& s, const int (&digit)[kItems], uint32_t (&rank)[kItems], int radix) {
+// lanes whose digit is this lane's
+__device__ __forceinline__ uint32_t digit_peers(uint32_t digit, bool there) { return __match_any_sync(0xffffffffu, there ? digit : kNoKey); }
+
+// Ranks of a tile's tokens among the tokens of the same digit, in the tile's order (the first `n` places hold one).  Afterwards
+// of_warp[w][d] holds the tokens of digit d in the warps before w, and sums[k] those of digit threadIdx.x + k * threads in the tile.
+template <int Warps, int Items>
+__device__ __forceinline__ void rank_tile(Counts<Warps>& s, const uint32_t (&key)[Items], int shift, int bits, int n, uint32_t (&rank)[Items],
+                                          uint32_t (&sums)[(kMaxRadix + Warps * 32 - 1) / (Warps * 32)]) {
+  constexpr int kAll = Warps * 32;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int i = threadIdx.x; i < kSortWarps * kMaxRadix / 2; i += kSortThreads) reinterpret_cast<uint32_t*>(s.warp_count)[i] = 0;
-  __syncthreads();
+  const uint32_t radix = 1u << bits;
+  for (uint32_t i = lane; i < radix; i += 32) s.of_warp[warp][i] = 0;
+  __syncwarp();
 #pragma unroll
-  for (int j = 0; j < kItems; ++j) {
-    const uint32_t peers = __match_any_sync(0xffffffffu, digit[j]);
-    const uint32_t before = peers & ((1u << lane) - 1u);
-    rank[j] = digit[j] < 0 ? 0u : s.warp_count[warp][digit[j]] + __popc(before);
+  for (int j = 0; j < Items; ++j) {
+    const uint32_t digit = key[j] >> shift & (radix - 1);
+    const bool there = tile_place<Items>(j) < n;
+    const uint32_t peers = digit_peers(digit, there), before = peers & ((1u << lane) - 1u);
+    const uint32_t upto = there ? s.of_warp[warp][digit] : 0u;
+    rank[j] = upto + __popc(before);
     __syncwarp();
-    if (digit[j] >= 0 && before == 0) s.warp_count[warp][digit[j]] += (uint16_t)__popc(peers);
+    if (there && before == 0) s.of_warp[warp][digit] = (uint16_t)(upto + __popc(peers));
     __syncwarp();
   }
   __syncthreads();
-  uint32_t sum = 0;
-  if (threadIdx.x < radix)
-    for (int w = 0; w < kSortWarps; ++w) {
-      const uint32_t c = s.warp_count[w][threadIdx.x];
-      s.warp_count[w][threadIdx.x] = (uint16_t)sum;
-      sum += c;
-    }
-  __syncthreads();
-  return sum;
+#pragma unroll
+  for (int k = 0; k < (kMaxRadix + kAll - 1) / kAll; ++k) {
+    const uint32_t d = threadIdx.x + k * kAll;
+    sums[k] = 0;
+    if (d < radix)
+#pragma unroll 8
+      for (int w = 0; w < Warps; ++w) {
+        const uint32_t c = s.of_warp[w][d];
+        s.of_warp[w][d] = (uint16_t)sums[k];
+        sums[k] += c;
+      }
+  }
 }
 
 // exclusive sum over the block's threads
-__device__ __forceinline__ uint32_t block_exclusive(SortShared& s, uint32_t x) {
+template <int Warps> __device__ __forceinline__ uint32_t block_exclusive(uint32_t* scan, uint32_t x) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint32_t sum = x;
 #pragma unroll
@@ -104,324 +169,465 @@ __device__ __forceinline__ uint32_t block_exclusive(SortShared& s, uint32_t x) {
     const uint32_t y = __shfl_up_sync(0xffffffffu, sum, d);
     if (lane >= d) sum += y;
   }
-  if (lane == 31) s.scan[warp] = sum;
+  if (lane == 31) scan[warp] = sum;
   __syncthreads();
   uint32_t before = 0;
-  for (int w = 0; w < warp; ++w) before += s.scan[w];
+#pragma unroll
+  for (int w = 0; w < Warps; ++w) before += w < warp ? scan[w] : 0u;
   __syncthreads();
   return before + sum - x;
 }
 
-// Every pass of the sort in one block, for at most kTile tokens.
-template <typename I>
-__global__ void __launch_bounds__(kSortThreads)
-embedding_sort_block_kernel(const I* __restrict__ index, int n, int64_t rows, int64_t padding, int passes, int bits,
-                            uint32_t* __restrict__ keys, uint32_t* __restrict__ tokens) {
-  extern __shared__ __align__(16) unsigned char smem[];
-  SortShared& s = *reinterpret_cast<SortShared*>(smem);
-  uint32_t* s_key = reinterpret_cast<uint32_t*>(smem + sizeof(SortShared));
-  uint32_t* s_token = s_key + kTile;
-  uint32_t key[kItems], token[kItems], rank[kItems];
-  int digit[kItems];
+// base[d]: tokens of smaller digits
+template <int Warps>
+__device__ __forceinline__ void digit_bases(Counts<Warps>& s, const uint32_t (&sums)[(kMaxRadix + Warps * 32 - 1) / (Warps * 32)], int bits) {
+  constexpr int kAll = Warps * 32;
+  uint32_t carry = 0;
 #pragma unroll
-  for (int j = 0; j < kItems; ++j) {
-    const int i = tile_place(j);
-    token[j] = i;
-    key[j] = i < n ? token_key(index[i], rows, padding) : 0xffffffffu;
-  }
-  const int radix = 1 << bits;
-  for (int pass = 0; pass < passes; ++pass) {
-#pragma unroll
-    for (int j = 0; j < kItems; ++j) digit[j] = tile_place(j) < n ? (int)((key[j] >> (pass * bits)) & (radix - 1)) : -1;
-    const uint32_t count = rank_tile(s, digit, rank, radix);
-    const uint32_t base = block_exclusive(s, count);
-    if (threadIdx.x < radix) s.base[threadIdx.x] = base;
-    __syncthreads();
-    const int warp = threadIdx.x >> 5;
-#pragma unroll
-    for (int j = 0; j < kItems; ++j)
-      if (digit[j] >= 0) {
-        const uint32_t at = s.base[digit[j]] + s.warp_count[warp][digit[j]] + rank[j];
-        s_key[at] = key[j];
-        s_token[at] = token[j];
-      }
-    __syncthreads();
-#pragma unroll
-    for (int j = 0; j < kItems; ++j) {
-      const int i = tile_place(j);
-      if (i < n) {
-        key[j] = s_key[i];
-        token[j] = s_token[i];
-      }
+  for (int k = 0; k < (kMaxRadix + kAll - 1) / kAll; ++k) {
+    const uint32_t d = threadIdx.x + k * kAll, at = block_exclusive<Warps>(s.scan, sums[k]);
+    if (d < (1u << bits)) s.base[d] = carry + at;
+    if (k + 1 < (kMaxRadix + kAll - 1) / kAll) {  // the next digits lie behind all of these
+      if (threadIdx.x == kAll - 1) s.scan[31] = at + sums[k];
+      __syncthreads();
+      carry += s.scan[31];
+      __syncthreads();
     }
   }
+  __syncthreads();
+}
+
+// Sorts up to Warps * 32 * Items tokens in the block; the result in shared memory, `keys` and `places` (token numbers).
+template <int Warps, int Items, typename Place>
+__device__ __forceinline__ void sort_block(Counts<Warps>& s, const Tokens& tokens, int passes, int bits, uint32_t* keys, Place* places) {
+  const int n = (int)tokens.n, warp = threadIdx.x >> 5;
+  uint32_t key[Items], place[Items], rank[Items], sums[(kMaxRadix + Warps * 32 - 1) / (Warps * 32)];
+  tokens.keys([](int j) { return (int64_t)tile_place<Items>(j); }, key);
 #pragma unroll
-  for (int j = 0; j < kItems; ++j) {
-    const int i = tile_place(j);
-    if (i < n) {
-      keys[i] = key[j];
-      tokens[i] = token[j];
+  for (int j = 0; j < Items; ++j) place[j] = tile_place<Items>(j);
+  for (int pass = 0; pass < passes; ++pass) {
+    rank_tile<Warps, Items>(s, key, pass * bits, bits, n, rank, sums);
+    digit_bases<Warps>(s, sums, bits);
+#pragma unroll
+    for (int j = 0; j < Items; ++j)
+      if (tile_place<Items>(j) < n) {
+        const uint32_t digit = key[j] >> (pass * bits) & ((1u << bits) - 1u);
+        const uint32_t at = s.base[digit] + s.of_warp[warp][digit] + rank[j];
+        keys[at] = key[j];
+        places[at] = (Place)place[j];
+      }
+    __syncthreads();
+    if (pass + 1 < passes) {
+#pragma unroll
+      for (int j = 0; j < Items; ++j) {
+        const int i = tile_place<Items>(j);
+        if (i < n) {
+          key[j] = keys[i];
+          place[j] = places[i];
+        }
+      }
+      __syncthreads();
     }
   }
 }
 
-// tokens of every digit in every tile: counts[digit][tile].  `index`: the first pass reads the indices themselves.
-template <typename I>
-__global__ void __launch_bounds__(kSortThreads)
-embedding_count_kernel(const I* __restrict__ index, const uint32_t* __restrict__ keys, int64_t n, int64_t rows, int64_t padding, int shift,
-                       int bits, uint32_t* __restrict__ counts, int n_tiles) {
+// A cluster of eight blocks sorts up to 65536 tokens in their shared memory: every block ranks its eighth, reads the others' digit
+// counts, and puts each token where it belongs, in whichever block that is.
+constexpr int kCluster = 8;
+constexpr int kClusterWarps = 32;
+constexpr int kClusterItems = 8;  // at most
+constexpr int kClusterSort = kCluster * kClusterWarps * 32 * kClusterItems;
+
+template <int Items> struct ClusterShared {
+  Counts<kClusterWarps> counts;
+  uint32_t totals[kMaxRadix];
+  uint32_t keys[2][kClusterWarps * 32 * Items], places[2][kClusterWarps * 32 * Items];
+};
+
+template <int Items>
+__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kClusterWarps * 32, 1)
+embedding_sort_cluster_kernel(Tokens tokens, int passes, int bits, uint32_t* __restrict__ out_keys, uint32_t* __restrict__ out_places) {
+  extern __shared__ __align__(16) unsigned char smem[];
+  ClusterShared<Items>& s = *reinterpret_cast<ClusterShared<Items>*>(smem);
+  constexpr int kMine = kClusterWarps * 32 * Items;
+  const cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
+  const int me = (int)cluster.block_rank(), warp = threadIdx.x >> 5;
+  const int64_t tile0 = (int64_t)me * kMine;
+  const int n = (int)max((int64_t)0, min((int64_t)kMine, tokens.n - tile0));
+  uint32_t key[Items], place[Items], rank[Items], sums[1];
+  tokens.keys([&](int j) { return tile0 + tile_place<Items>(j); }, key);
+#pragma unroll
+  for (int j = 0; j < Items; ++j) place[j] = (uint32_t)(tile0 + tile_place<Items>(j));
+  for (int pass = 0; pass < passes; ++pass) {
+    const int shift = pass * bits;
+    rank_tile<kClusterWarps, Items>(s.counts, key, shift, bits, n, rank, sums);
+    if (threadIdx.x < (1u << bits)) s.totals[threadIdx.x] = sums[0];
+    cluster.sync();
+    uint32_t before = 0, all = 0;
+    if (threadIdx.x < (1u << bits)) {
+#pragma unroll
+      for (int c = 0; c < kCluster; ++c) {
+        const uint32_t there = cluster.map_shared_rank(s.totals, c)[threadIdx.x];
+        if (c < me) before += there;
+        all += there;
+      }
+    }
+    const uint32_t base = block_exclusive<kClusterWarps>(s.counts.scan, all);
+    if (threadIdx.x < (1u << bits)) s.counts.base[threadIdx.x] = base + before;
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < Items; ++j)
+      if (tile_place<Items>(j) < n) {
+        const uint32_t digit = key[j] >> shift & ((1u << bits) - 1u);
+        const uint32_t at = s.counts.base[digit] + s.counts.of_warp[warp][digit] + rank[j];
+        cluster.map_shared_rank(s.keys[pass & 1], at / kMine)[at % kMine] = key[j];
+        cluster.map_shared_rank(s.places[pass & 1], at / kMine)[at % kMine] = place[j];
+      }
+    cluster.sync();
+    if (pass + 1 < passes) {
+#pragma unroll
+      for (int j = 0; j < Items; ++j) {
+        const int i = tile_place<Items>(j);
+        key[j] = i < n ? s.keys[pass & 1][i] : 0u;
+        place[j] = i < n ? s.places[pass & 1][i] : 0u;
+      }
+    }
+  }
+  for (int i = threadIdx.x; i < n; i += kClusterWarps * 32) {
+    out_keys[tile0 + i] = s.keys[(passes - 1) & 1][i];
+    out_places[tile0 + i] = s.places[(passes - 1) & 1][i];
+  }
+}
+
+constexpr int kTileWarps = 16;
+constexpr int kItems = 8;
+constexpr int kTile = kTileWarps * 32 * kItems;  // tokens of a tile
+
+// keys of a tile; `sorted` null: from the indices
+__device__ __forceinline__ void tile_keys(const Tokens& tokens, const uint32_t* sorted, int64_t tile0, uint32_t (&key)[kItems]) {
+  if (sorted) {
+#pragma unroll
+    for (int j = 0; j < kItems; ++j) {
+      const int64_t i = tile0 + tile_place<kItems>(j);
+      key[j] = i < tokens.n ? sorted[i] : 0u;
+    }
+  } else {
+    tokens.keys([&](int j) { return tile0 + tile_place<kItems>(j); }, key);
+  }
+}
+
+// tokens of every digit in every tile: counts[digit][tile].  `keys` null: the first pass, which reads the indices.
+__global__ void __launch_bounds__(kTileWarps * 32)
+embedding_count_kernel(Tokens tokens, const uint32_t* __restrict__ keys, int shift, int bits, uint32_t* __restrict__ counts, int n_tiles) {
   __shared__ uint32_t s_count[kMaxRadix];
-  const int radix = 1 << bits;
+  const uint32_t radix = 1u << bits;
+  for (uint32_t d = threadIdx.x; d < radix; d += kTileWarps * 32) s_count[d] = 0;
   griddep_wait();
-  for (int d = threadIdx.x; d < radix; d += kSortThreads) s_count[d] = 0;
-  __syncthreads();
   const int64_t tile0 = (int64_t)blockIdx.x * kTile;
+  uint32_t key[kItems];
+  tile_keys(tokens, keys, tile0, key);
+  __syncthreads();
 #pragma unroll
   for (int j = 0; j < kItems; ++j) {
-    const int64_t i = tile0 + tile_place(j);
-    int d = -1;
-    if (i < n) d = (int)(((index ? token_key(index[i], rows, padding) : keys[i]) >> shift) & (radix - 1));
-    const uint32_t peers = __match_any_sync(0xffffffffu, d);
-    if (d >= 0 && (peers & ((1u << (threadIdx.x & 31)) - 1u)) == 0) atomicAdd(&s_count[d], __popc(peers));
+    const bool there = tile0 + tile_place<kItems>(j) < tokens.n;
+    const uint32_t digit = key[j] >> shift & (radix - 1);
+    const uint32_t peers = digit_peers(digit, there);
+    if (there && (peers & ((1u << (threadIdx.x & 31)) - 1u)) == 0) atomicAdd(&s_count[digit], __popc(peers));
   }
   __syncthreads();
-  for (int d = threadIdx.x; d < radix; d += kSortThreads) counts[(int64_t)d * n_tiles + blockIdx.x] = s_count[d];
+  for (uint32_t d = threadIdx.x; d < radix; d += kTileWarps * 32) counts[(int64_t)d * n_tiles + blockIdx.x] = s_count[d];
 }
 
 // One block per digit: its counts become the tokens of that digit in the tiles before, and totals[digit] their sum.
 __global__ void __launch_bounds__(kThreads) embedding_scan_kernel(uint32_t* __restrict__ counts, int n_tiles, uint32_t* __restrict__ totals) {
-  __shared__ uint32_t s_sum[kThreads / 32];
+  __shared__ uint32_t s_scan[kThreads / 32], s_sum;
   griddep_wait();
   uint32_t* row = counts + (int64_t)blockIdx.x * n_tiles;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint32_t carry = 0;
   for (int first = 0; first < n_tiles; first += kThreads) {
     const int i = first + threadIdx.x;
     const uint32_t x = i < n_tiles ? row[i] : 0u;
-    uint32_t sum = x;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const uint32_t y = __shfl_up_sync(0xffffffffu, sum, d);
-      if (lane >= d) sum += y;
-    }
-    if (lane == 31) s_sum[warp] = sum;
+    const uint32_t before = block_exclusive<kThreads / 32>(s_scan, x);
+    if (i < n_tiles) row[i] = carry + before;
+    if (threadIdx.x == kThreads - 1) s_sum = before + x;
     __syncthreads();
-    uint32_t before = 0, all = 0;
-    for (int w = 0; w < kThreads / 32; ++w) {
-      if (w < warp) before += s_sum[w];
-      all += s_sum[w];
-    }
-    if (i < n_tiles) row[i] = carry + before + sum - x;
-    carry += all;
+    carry += s_sum;
     __syncthreads();
   }
   if (threadIdx.x == 0) totals[blockIdx.x] = carry;
 }
 
-template <typename I>
-__global__ void __launch_bounds__(kSortThreads)
-embedding_scatter_kernel(const I* __restrict__ index, const uint32_t* __restrict__ keys, const uint32_t* __restrict__ tokens, int64_t n,
-                         int64_t rows, int64_t padding, int shift, int bits, const uint32_t* __restrict__ counts,
-                         const uint32_t* __restrict__ totals, int n_tiles, uint32_t* __restrict__ out_keys,
-                         uint32_t* __restrict__ out_tokens) {
-  __shared__ SortShared s;
+__global__ void __launch_bounds__(kTileWarps * 32)
+embedding_scatter_kernel(Tokens tokens, const uint32_t* __restrict__ keys, const uint32_t* __restrict__ places, int shift, int bits,
+                         const uint32_t* __restrict__ counts, const uint32_t* __restrict__ totals, int n_tiles, uint32_t* __restrict__ out_keys,
+                         uint32_t* __restrict__ out_places) {
+  __shared__ Counts<kTileWarps> s;
   griddep_wait();
-  const int radix = 1 << bits;
+  const uint32_t radix = 1u << bits;
   const int64_t tile0 = (int64_t)blockIdx.x * kTile;
-  uint32_t key[kItems], token[kItems], rank[kItems];
-  int digit[kItems];
+  const int n = (int)min((int64_t)kTile, tokens.n - tile0);
+  const uint32_t total = threadIdx.x < radix ? totals[threadIdx.x] : 0u;
+  const uint32_t here = threadIdx.x < radix ? counts[(int64_t)threadIdx.x * n_tiles + blockIdx.x] : 0u;
+  uint32_t key[kItems], place[kItems], rank[kItems], sums[1];
+  tile_keys(tokens, keys, tile0, key);
 #pragma unroll
-  for (int j = 0; j < kItems; ++j) {
-    const int64_t i = tile0 + tile_place(j);
-    digit[j] = -1;
-    if (i < n) {
-      key[j] = index ? token_key(index[i], rows, padding) : keys[i];
-      token[j] = index ? (uint32_t)i : tokens[i];
-      digit[j] = (int)((key[j] >> shift) & (radix - 1));
-    }
+  for (int j = 0; j < kItems; ++j) place[j] = (uint32_t)(tile0 + tile_place<kItems>(j));
+  if (keys) {
+#pragma unroll
+    for (int j = 0; j < kItems; ++j) place[j] = place[j] < tokens.n ? places[place[j]] : 0u;
   }
-  rank_tile(s, digit, rank, radix);
-  const uint32_t base = block_exclusive(s, threadIdx.x < radix ? totals[threadIdx.x] : 0u);
-  if (threadIdx.x < radix) s.base[threadIdx.x] = base + counts[(int64_t)threadIdx.x * n_tiles + blockIdx.x];
+  rank_tile<kTileWarps, kItems>(s, key, shift, bits, n, rank, sums);
+  const uint32_t base = block_exclusive<kTileWarps>(s.scan, total);
+  if (threadIdx.x < radix) s.base[threadIdx.x] = base + here;
   __syncthreads();
   const int warp = threadIdx.x >> 5;
 #pragma unroll
   for (int j = 0; j < kItems; ++j)
-    if (digit[j] >= 0) {
-      const uint32_t at = s.base[digit[j]] + s.warp_count[warp][digit[j]] + rank[j];
+    if (tile_place<kItems>(j) < n) {
+      const uint32_t digit = key[j] >> shift & (radix - 1);
+      const uint32_t at = s.base[digit] + s.of_warp[warp][digit] + rank[j];
       out_keys[at] = key[j];
-      out_tokens[at] = token[j];
+      out_places[at] = place[j];
     }
 }
 
 // ---- sums ----------------------------------------------------------------------------------------------------------
 
+constexpr int kSpan = 2048;               // sorted tokens of a block, at most
+constexpr int kLocalItems = 4;
+constexpr int kLocal = kThreads * kLocalItems;  // tokens that every block sorts itself
+constexpr int kFillRows = 1024;           // rows of a block that fills, at most
+
 struct SumArgs {
+  Tokens tokens;           // `local`: sorted in the block
+  int local, passes, bits;
+  const uint32_t* keys;    // else sorted before; entries of key `rows` are left out
+  const uint32_t* places;
   const void* grad;
   int64_t grad_stride;
   void* out;
   int64_t out_stride;
-  const uint32_t* keys;    // sorted; entries of key `rows` are left out
-  const uint32_t* tokens;
-  int64_t n, rows;
   int dim, lanes, n_cols;  // lanes: pieces of a row that a block's worker takes, n_cols such parts make a row
   int workers;             // workers of a block
   int share;               // sorted tokens of a worker
   int64_t n_blocks;        // blocks along the tokens
-  float* pieces;           // [n_blocks][2][padded dim]: the sum that a block's first row had before its first token's share ...
-  int64_t piece_stride;    // ... (the row began in an earlier block), and that of a row that ends in a later one
+  // Pieces [n_blocks][2][piece_stride] of the rows that blocks share: the sum of a block's tokens of the row that an earlier block began
+  // (its key in keys_of[2 * block], else `rows`), and of the row that goes on in a later block and began in this one.
+  float* pieces;
+  uint32_t* keys_of;
+  int64_t piece_stride;
   float scale;
-  int accumulate;
-  int64_t fill_rows;       // rows of a block that writes the rows without a token, 0: none does
+  int fill_rows;           // rows of a block that fills rows without a token with zeros, 0: there are none
 };
 
-template <typename TO, int N> __device__ __forceinline__ void write_row(const SumArgs& a, uint32_t row, int64_t c, const float (&x)[N]) {
-  Pack<TO, N>* at = reinterpret_cast<Pack<TO, N>*>(static_cast<TO*>(a.out) + (int64_t)row * a.out_stride + c);
-  Pack<TO, N> y;
-  if (a.accumulate) {
-    const Pack<TO, N> old = *at;
-#pragma unroll
-    for (int k = 0; k < N; ++k) y.v[k] = from_float<TO>(fmaf(x[k], a.scale, to_float(old.v[k])));
-  } else {
-#pragma unroll
-    for (int k = 0; k < N; ++k) y.v[k] = from_float<TO>(x[k] * a.scale);
-  }
-  *at = y;
+template <typename TO, int N> __device__ __forceinline__ TO* row_at(const SumArgs& a, uint32_t row, int64_t c) {
+  return static_cast<TO*>(a.out) + (int64_t)row * a.out_stride + c;
 }
 
-template <int N> __device__ __forceinline__ float* piece_at(const SumArgs& a, int64_t block, int which, int64_t c) {
+// scale * x, added to what was there with Add
+template <typename TO, int N, bool Add> __device__ __forceinline__ void write_row(const SumArgs& a, TO* at, const float (&x)[N], const Raw<TO, N>& old) {
+  Pack<TO, N> y;
+#pragma unroll
+  for (int k = 0; k < N; ++k) y.v[k] = from_float<TO>(Add ? fmaf(x[k], a.scale, old.get(k)) : x[k] * a.scale);
+  *reinterpret_cast<Pack<TO, N>*>(at) = y;
+}
+template <typename TO, int N, bool Add> __device__ __forceinline__ void write_row(const SumArgs& a, uint32_t row, int64_t c, const float (&x)[N]) {
+  TO* at = row_at<TO, N>(a, row, c);
+  Raw<TO, N> old{};
+  if (Add) old.load(at);
+  write_row<TO, N, Add>(a, at, x, old);
+}
+
+__device__ __forceinline__ float* piece_at(const SumArgs& a, int64_t block, int which, int64_t c) {
   return a.pieces + (block * 2 + which) * a.piece_stride + c;
 }
 
-// first position of the sorted keys that is not below `key`
-__device__ __forceinline__ int64_t lower_bound(const uint32_t* keys, int64_t n, uint32_t key) {
+// first position of the sorted keys that is not below `key`, found by a warp
+__device__ __forceinline__ int64_t warp_lower_bound(const uint32_t* keys, int64_t n, uint32_t key) {
   int64_t lo = 0, hi = n;
   while (lo < hi) {
-    const int64_t mid = (lo + hi) >> 1;
-    if (keys[mid] < key) lo = mid + 1;
-    else hi = mid;
+    const int64_t step = (hi - lo + 32) / 33, at = lo + ((threadIdx.x & 31) + 1) * step - 1;
+    const int below = __popc(__ballot_sync(0xffffffffu, at < hi && keys[at] < key));
+    lo += below * step;
+    hi = min(hi, lo + step - 1);
   }
   return lo;
 }
 
-// zeros in the rows that no token names
-template <typename TO, int N> __device__ __forceinline__ void fill_rows(const SumArgs& a, int64_t first) {
-  __shared__ uint32_t s_named[kThreads / 32];
-  const int64_t last = min(first + a.fill_rows, a.rows);
-  if (threadIdx.x < kThreads / 32) s_named[threadIdx.x] = 0;
-  __syncthreads();
-  if (threadIdx.x < last - first) {
-    const uint32_t row = (uint32_t)(first + threadIdx.x);
-    const int64_t at = lower_bound(a.keys, a.n, row);
-    if (at < a.n && a.keys[at] == row) atomicOr(&s_named[threadIdx.x >> 5], 1u << (threadIdx.x & 31));
+// zeros in those rows from `first` on that no token names
+template <typename TO> __device__ __forceinline__ void fill_rows(const SumArgs& a, int64_t first, uint32_t* named, int64_t* range) {
+  const int64_t last = min(first + a.fill_rows, a.tokens.rows);
+  for (int i = threadIdx.x; i < kFillRows / 32; i += kThreads) named[i] = 0;
+  if (!a.local && threadIdx.x < 64) {
+    const int64_t at = warp_lower_bound(a.keys, a.tokens.n, (uint32_t)(threadIdx.x < 32 ? first : last));
+    range[threadIdx.x >> 5] = at;
   }
   __syncthreads();
-  const int per_row = a.dim / N;
-  Pack<TO, N> zero;
-#pragma unroll
-  for (int k = 0; k < N; ++k) zero.v[k] = from_float<TO>(0.0f);
-  for (int64_t row = first; row < last; ++row) {
-    const int r = (int)(row - first);
-    if (s_named[r >> 5] >> (r & 31) & 1u) continue;
-    for (int c = threadIdx.x; c < per_row; c += kThreads)
-      *reinterpret_cast<Pack<TO, N>*>(static_cast<TO*>(a.out) + row * a.out_stride + (int64_t)c * N) = zero;
+  const int64_t lo = a.local ? 0 : range[0], hi = a.local ? a.tokens.n : range[1];
+  if (hi - lo <= 4096) {  // few tokens: all of them, the first of a row marking it
+    for (int64_t i = lo + threadIdx.x; i < hi; i += kThreads) {
+      const uint32_t key = a.local ? a.tokens.key(i) : a.keys[i];
+      if (key >= first && key < last && (a.local || i == lo || a.keys[i - 1] != key)) atomicOr(&named[(key - first) >> 5], 1u << ((key - first) & 31));
+    }
+  } else {  // many: a search for every row
+    for (int r = threadIdx.x; r < last - first; r += kThreads) {
+      const uint32_t key = (uint32_t)(first + r);
+      int64_t from = lo, to = hi;
+      while (from < to) {
+        const int64_t mid = (from + to) >> 1;
+        if (a.keys[mid] < key) from = mid + 1;
+        else to = mid;
+      }
+      if (from < hi && a.keys[from] == key) atomicOr(&named[r >> 5], 1u << (r & 31));
+    }
+  }
+  __syncthreads();
+  TO* out = static_cast<TO*>(a.out) + first * a.out_stride;
+  const uint4 zero = make_uint4(0, 0, 0, 0);
+  constexpr int kWide = 16 / sizeof(TO);
+  if (a.out_stride == a.dim && a.dim % kWide == 0 && (uintptr_t)a.out % 16 == 0) {
+    const uint32_t per_row = a.dim / kWide, all = (uint32_t)(last - first) * per_row;
+    for (uint32_t i = threadIdx.x; i < all; i += kThreads) {
+      const uint32_t r = i / per_row;
+      if (!(named[r >> 5] >> (r & 31) & 1u)) reinterpret_cast<uint4*>(out)[i] = zero;
+    }
+  } else {  // a warp to a row: single values up to a 16-byte boundary, 16 bytes at a time, single values
+    for (int r = threadIdx.x >> 5; r < last - first; r += kThreads / 32) {
+      if (named[r >> 5] >> (r & 31) & 1u) continue;
+      TO* row = out + (int64_t)r * a.out_stride;
+      const int lane = threadIdx.x & 31;
+      const int head = min(a.dim, (int)((16 - (uintptr_t)row % 16) % 16 / sizeof(TO))), body = (a.dim - head) / kWide;
+      if (lane < head) row[lane] = from_float<TO>(0.0f);
+      for (int i = lane; i < body; i += 32) reinterpret_cast<uint4*>(row + head)[i] = zero;
+      const int tail = head + body * kWide + lane;
+      if (tail < a.dim) row[tail] = from_float<TO>(0.0f);
+    }
   }
 }
 
-constexpr int kBatch = 8;  // rows in flight per worker
+template <int N> struct SumShared {
+  union {
+    Counts<kThreads / 32> sort;
+    struct {
+      float head[kThreads][N], tail[kThreads][N];
+    };
+  };
+  int through[kThreads];      // the whole share is one row that began before it and goes on behind it
+  uint32_t key[kSpan + 2];    // of the tokens before, of and behind the block
+  uint32_t token[kSpan];
+  int valid;                  // tokens of the block that are summed
+  uint32_t named[kFillRows / 32];
+  int64_t range[2];
+};
 
-template <typename TI, typename TO, int N> __global__ void __launch_bounds__(kThreads) embedding_sum_kernel(SumArgs a) {
-  __shared__ float s_head[kThreads][N], s_tail[kThreads][N];
-  __shared__ uint32_t s_tail_key[kThreads];  // key of the row that goes on behind a worker's share, or `rows`
-  __shared__ int s_through[kThreads];        // the whole share is one row that began before it and goes on behind it
+template <typename TI, typename TO, int N, bool Add> __global__ void __launch_bounds__(kThreads) embedding_sum_kernel(SumArgs a) {
+  __shared__ SumShared<N> s;
+  constexpr int kBatch = Add ? 4 : 8;  // rows in flight
   griddep_wait();
   const int64_t sum_blocks = a.n_blocks * a.n_cols;
   if (blockIdx.x >= sum_blocks) {
-    fill_rows<TO, N>(a, ((int64_t)blockIdx.x - sum_blocks) * a.fill_rows);
+    fill_rows<TO>(a, ((int64_t)blockIdx.x - sum_blocks) * a.fill_rows, s.named, s.range);
     return;
   }
-  const int64_t block = blockIdx.x / a.n_cols;
+  const int64_t block = blockIdx.x / a.n_cols, block0 = block * a.workers * a.share;
+  const int count = (int)min((int64_t)a.workers * a.share, a.tokens.n - block0);
+  const uint32_t none = (uint32_t)a.tokens.rows;
+  if (threadIdx.x == 0) s.valid = 0;
+  int off = 0;  // of the block's first token in s.token, and in s.key of the token before it
+  if (a.local) {
+    off = (int)block0;
+    sort_block<kThreads / 32, kLocalItems>(s.sort, a.tokens, a.passes, a.bits, s.key + 1, s.token);
+    if (threadIdx.x == 0) s.key[0] = s.key[a.tokens.n + 1] = kNoKey;
+  } else {
+    for (int i = threadIdx.x; i < count; i += kThreads) {
+      s.key[i + 1] = a.keys[block0 + i];
+      s.token[i] = a.places[block0 + i];
+    }
+    if (threadIdx.x == 0) s.key[0] = block0 > 0 ? a.keys[block0 - 1] : kNoKey;
+    if (threadIdx.x == 1) s.key[count + 1] = block0 + count < a.tokens.n ? a.keys[block0 + count] : kNoKey;
+  }
+  __syncthreads();
+  const uint32_t* keys = s.key + off + 1;  // keys[-1]: before the block
+  const uint32_t* tokens = s.token + off;
+  for (int i = threadIdx.x; i < count; i += kThreads)  // tokens that are left out lie behind all others
+    if (keys[i] != none && (i + 1 == count || keys[i + 1] == none)) s.valid = i + 1;
+  __syncthreads();
   const int worker = threadIdx.x / a.lanes;
   const int piece = (int)(blockIdx.x % a.n_cols) * a.lanes + (int)threadIdx.x % a.lanes;
-  const bool on = worker < a.workers && piece * N < a.dim;
+  const bool on = worker < a.workers && (int64_t)piece * N < a.dim;
   const int64_t c = (int64_t)piece * N;
-  const uint32_t none = (uint32_t)a.rows;
-  const int64_t begin = (block * a.workers + worker) * a.share, end = min(begin + a.share, a.n);
+  const int begin = worker * a.share, end = min(begin + a.share, s.valid);
   const TI* grad = static_cast<const TI*>(a.grad) + c;
-  uint32_t tail_key = none, head_key = none;
-  bool through = false;
+  bool through = false, tail = false;
   if (on && begin < end) {
-    uint32_t cur = a.keys[begin];
-    bool first = begin > 0 && a.keys[begin - 1] == cur;  // this row began before the share
-    if (first) head_key = cur;
+    bool first = keys[begin - 1] == keys[begin];  // the row that began before the share
     float acc[N];
 #pragma unroll
     for (int k = 0; k < N; ++k) acc[k] = 0.0f;
-    for (int64_t i = begin; i < end; i += kBatch) {
-      uint32_t key[kBatch];
-      Pack<TI, N> x[kBatch];
+    for (int i = begin; i < end; i += kBatch) {
+      Raw<TI, N> x[kBatch];
+      Raw<TO, N> old[Add ? kBatch : 1];
 #pragma unroll
-      for (int b = 0; b < kBatch; ++b) {
-        key[b] = i + b < end ? a.keys[i + b] : none;
-        if (key[b] != none) x[b] = *reinterpret_cast<const Pack<TI, N>*>(grad + (int64_t)a.tokens[i + b] * a.grad_stride);
+      for (int b = 0; b < kBatch; ++b) x[b].load(grad + (int64_t)tokens[min(i + b, end - 1)] * a.grad_stride);
+      if constexpr (Add) {
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b)
+          if (i + b < end && keys[i + b + 1] != keys[i + b]) old[b].load(row_at<TO, N>(a, keys[i + b], c));
       }
 #pragma unroll
       for (int b = 0; b < kBatch; ++b) {
         if (i + b >= end) break;
-        if (key[b] != cur) {
+        const uint32_t key = keys[i + b];
+#pragma unroll
+        for (int k = 0; k < N; ++k) acc[k] += x[b].get(k);
+        if (keys[i + b + 1] != key) {  // the row ends
           if (first) {
 #pragma unroll
-            for (int k = 0; k < N; ++k) s_head[threadIdx.x][k] = acc[k];
-          } else if (cur != none) {
-            write_row<TO, N>(a, cur, c, acc);
+            for (int k = 0; k < N; ++k) s.head[threadIdx.x][k] = acc[k];
+          } else {
+            write_row<TO, N, Add>(a, row_at<TO, N>(a, key, c), acc, old[Add ? b : 0]);
           }
           first = false;
-          cur = key[b];
 #pragma unroll
           for (int k = 0; k < N; ++k) acc[k] = 0.0f;
         }
-        if (cur != none) {
-#pragma unroll
-          for (int k = 0; k < N; ++k) acc[k] += to_float(x[b].v[k]);
-        }
       }
     }
-    const bool goes_on = cur != none && end < a.n && a.keys[end] == cur;
-    if (first) {
+    if (keys[end] == keys[end - 1]) {  // the last row goes on
+      through = first;
+      tail = !first;
 #pragma unroll
-      for (int k = 0; k < N; ++k) s_head[threadIdx.x][k] = acc[k];
-      through = goes_on;
-    } else if (goes_on) {
-#pragma unroll
-      for (int k = 0; k < N; ++k) s_tail[threadIdx.x][k] = acc[k];
-      tail_key = cur;
-    } else if (cur != none) {
-      write_row<TO, N>(a, cur, c, acc);
+      for (int k = 0; k < N; ++k) (first ? s.head : s.tail)[threadIdx.x][k] = acc[k];
     }
   }
-  s_tail_key[threadIdx.x] = tail_key;
-  s_through[threadIdx.x] = through;
+  s.through[threadIdx.x] = through;
   __syncthreads();
+  const bool from_before = keys[0] != none && keys[-1] == keys[0];
+  if (threadIdx.x == 0 && blockIdx.x % a.n_cols == 0 && a.n_blocks > 1) {
+    const uint32_t last = keys[count - 1];
+    a.keys_of[2 * block] = from_before ? keys[0] : none;
+    a.keys_of[2 * block + 1] = last != none && keys[count] == last && !(from_before && keys[0] == last) ? last : none;
+  }
   if (!on) return;
   // A row that goes on behind a worker's share is joined by the worker it begins with; the one that came from the block
   // before by the first.
-  const bool from_before = worker == 0 && head_key != none;
   for (int kind = 0; kind < 2; ++kind) {
-    if (kind == 0 ? !from_before : tail_key == none) continue;
+    if (kind == 0 ? worker != 0 || !from_before : !tail) continue;
     float acc[N];
 #pragma unroll
-    for (int k = 0; k < N; ++k) acc[k] = kind == 0 ? s_head[threadIdx.x][k] : s_tail[threadIdx.x][k];
+    for (int k = 0; k < N; ++k) acc[k] = (kind == 0 ? s.head : s.tail)[threadIdx.x][k];
     bool open = kind == 0 ? through : true;
     for (int w = worker + 1; open && w < a.workers; ++w) {
       const int t = w * a.lanes + (int)threadIdx.x % a.lanes;
+      if (w * a.share >= count) break;  // it goes on in the next block
 #pragma unroll
-      for (int k = 0; k < N; ++k) acc[k] += s_head[t][k];
-      open = s_through[t];
+      for (int k = 0; k < N; ++k) acc[k] += s.head[t][k];
+      open = s.through[t];
     }
     if (kind == 1 && !open) {
-      write_row<TO, N>(a, tail_key, c, acc);
+      write_row<TO, N, Add>(a, keys[end - 1], c, acc);
     } else {
-      float* at = piece_at<N>(a, block, kind, c);
+      float* at = piece_at(a, block, kind, c);
 #pragma unroll
       for (int k = 0; k < N; ++k) at[k] = acc[k];
     }
@@ -429,37 +635,32 @@ template <typename TI, typename TO, int N> __global__ void __launch_bounds__(kTh
 }
 
 // Rows that several blocks share: the block that one begins in adds the others' pieces, its workers equal shares of them.
-template <typename TO, int N> __global__ void __launch_bounds__(kThreads) embedding_join_kernel(SumArgs a) {
+template <typename TO, int N, bool Add> __global__ void __launch_bounds__(kThreads) embedding_join_kernel(SumArgs a) {
   __shared__ float s_sum[kThreads][N];
   griddep_wait();
   const int64_t block = blockIdx.x / a.n_cols;
-  const int64_t span = (int64_t)a.workers * a.share;
-  const int64_t begin = block * span, end = begin + span;
-  if (end >= a.n) return;
-  const uint32_t key = a.keys[end];
-  if (key == (uint32_t)a.rows || a.keys[end - 1] != key) return;
-  if (begin > 0 && a.keys[begin - 1] == key) return;  // it began before this block
-  // blocks whose first token is of this row: [block + 1, last)
-  int64_t lo = block + 1, hi = a.n_blocks;
-  while (lo < hi) {
-    const int64_t mid = (lo + hi) >> 1;
-    if (a.keys[mid * span] == key) lo = mid + 1;
-    else hi = mid;
+  const uint32_t key = a.keys_of[2 * block + 1];
+  if (key == (uint32_t)a.tokens.rows) return;
+  int64_t count = 0;  // blocks behind this one that go on with the row
+  for (bool more = true; more;) {
+    const int64_t b = block + 1 + count + threadIdx.x;
+    const int found = __syncthreads_count(b < a.n_blocks && a.keys_of[2 * b] == key);
+    count += found;
+    more = found == kThreads;
   }
-  const int64_t count = lo - (block + 1);
   const int worker = threadIdx.x / a.lanes;
   const int piece = (int)(blockIdx.x % a.n_cols) * a.lanes + (int)threadIdx.x % a.lanes;
-  const bool on = worker < a.workers && piece * N < a.dim;
+  const bool on = worker < a.workers && (int64_t)piece * N < a.dim;
   const int64_t c = (int64_t)piece * N;
   const int64_t each = (count + a.workers - 1) / a.workers;
-  const int64_t first = block + 1 + min(worker * each, count), last = block + 1 + min((worker + 1) * each, count);
+  const int64_t from = block + 1 + min(worker * each, count), to = block + 1 + min((worker + 1) * each, count);
   float acc[N];
 #pragma unroll
-  for (int k = 0; k < N; ++k) acc[k] = on && worker == 0 ? piece_at<N>(a, block, 1, c)[k] : 0.0f;
+  for (int k = 0; k < N; ++k) acc[k] = on && worker == 0 ? piece_at(a, block, 1, c)[k] : 0.0f;
   if (on) {
 #pragma unroll 8
-    for (int64_t b = first; b < last; ++b) {
-      const float* at = piece_at<N>(a, b, 0, c);
+    for (int64_t b = from; b < to; ++b) {
+      const float* at = piece_at(a, b, 0, c);
 #pragma unroll
       for (int k = 0; k < N; ++k) acc[k] += at[k];
     }
@@ -471,7 +672,7 @@ template <typename TO, int N> __global__ void __launch_bounds__(kThreads) embedd
   for (int w = 1; w < a.workers && w * each < count; ++w)
 #pragma unroll
     for (int k = 0; k < N; ++k) acc[k] += s_sum[w * a.lanes + threadIdx.x][k];
-  write_row<TO, N>(a, key, c, acc);
+  write_row<TO, N, Add>(a, key, c, acc);
 }
 
 // ---- plan ----------------------------------------------------------------------------------------------------------
@@ -480,24 +681,23 @@ size_t align256(size_t v) { return (v + 255) / 256 * 256; }
 
 // Everything that the sizes decide.
 struct GradPlan {
-  int n_values;            // values of a piece
   int lanes, n_cols, workers, share;
   int64_t n_blocks, piece_stride;
   int passes, bits, n_tiles;
-  size_t keys[2], tokens[2], counts, totals, pieces, total;
+  size_t keys[2], places[2], counts, totals, pieces, keys_of, total;
 };
 
 GradPlan grad_plan(int64_t n, int64_t rows, int dim, int n_values) {
   GradPlan p{};
-  p.n_values = n_values;
   const int per_row = (dim + n_values - 1) / n_values;
   p.lanes = std::min(per_row, kThreads);
   p.n_cols = (per_row + p.lanes - 1) / p.lanes;
   p.workers = kThreads / p.lanes;
-  // as many tokens to a worker as let the threads of one wave of full SMs cover them, at least two batches
+  // as many tokens to a worker as let two waves of half-full SMs cover them; one block where that is not far off
   const int64_t wave = (int64_t)GNR_SM_COUNT_FALLBACK * 2048;
-  const int64_t share = (n * p.lanes * p.n_cols + wave - 1) / wave;
-  p.share = (int)std::max<int64_t>(2 * kBatch, (share + kBatch - 1) / kBatch * kBatch);
+  int64_t share = std::max<int64_t>(16, (n * p.lanes * p.n_cols + wave - 1) / wave);
+  if (n <= (int64_t)p.workers * 32) share = std::max<int64_t>(1, (n + p.workers - 1) / p.workers);
+  p.share = (int)std::min<int64_t>((share + 7) / 8 * 8, std::max(8, kSpan / p.workers / 8 * 8));
   const int64_t span = (int64_t)p.share * p.workers;
   p.n_blocks = (n + span - 1) / span;
   p.piece_stride = (int64_t)per_row * n_values;
@@ -512,13 +712,19 @@ GradPlan grad_plan(int64_t n, int64_t rows, int dim, int n_values) {
     at += align256(bytes);
     return here;
   };
-  for (int k = 0; k < 2; ++k) {
-    p.keys[k] = take((size_t)n * 4);
-    p.tokens[k] = take((size_t)n * 4);
+  if (n > kLocal)
+    for (int k = 0; k < (n > kClusterSort ? 2 : 1); ++k) {
+      p.keys[k] = take((size_t)n * 4);
+      p.places[k] = take((size_t)n * 4);
+    }
+  if (n > kClusterSort) {
+    p.counts = take((size_t)p.n_tiles * kMaxRadix * 4);
+    p.totals = take(kMaxRadix * 4);
   }
-  p.counts = take((size_t)p.n_tiles * kMaxRadix * 4);
-  p.totals = take(kMaxRadix * 4);
-  p.pieces = take((size_t)p.n_blocks * 2 * p.piece_stride * 4);
+  if (p.n_blocks > 1) {
+    p.pieces = take((size_t)p.n_blocks * 2 * p.piece_stride * 4);
+    p.keys_of = take((size_t)p.n_blocks * 2 * 4);
+  }
   p.total = at;
   return p;
 }
@@ -553,10 +759,12 @@ extern "C" int gnr_embedding_lookup(const void* table, int type, int64_t rows, i
     return -1;
   }
   const cudaStream_t st = (cudaStream_t)stream;
-  const int size = gnr_type_size(type), wide = 16 / size;
-  const bool vec = dim % wide == 0 && aligned(table, table_stride, size, 16) && aligned(out, out_stride, size, 16);
-  const int per_row = vec ? dim / wide : dim;
-  const int64_t pieces = n * per_row, blocks = (pieces + kThreads - 1) / kThreads;
+  const int size = gnr_type_size(type);
+  // pieces of 32 bytes, 16 or one value
+  auto fits = [&](int to) { return (int64_t)dim * size % to == 0 && aligned(table, table_stride, size, to) && aligned(out, out_stride, size, to); };
+  const int piece = fits(32) ? 32 / size : fits(16) ? 16 / size : 1;
+  const uint32_t per_row = (uint32_t)(dim / piece);
+  const int64_t blocks = (n * per_row + kThreads * kPieces - 1) / (kThreads * kPieces);
   if (blocks > 0x7fffffff) {
     gnr_set_error("gnr_embedding_lookup: %lld values are too many for one call", (long long)(n * dim));
     return -1;
@@ -565,13 +773,10 @@ extern "C" int gnr_embedding_lookup(const void* table, int type, int64_t rows, i
     using T = decltype(t);
     constexpr int N = 16 / sizeof(T);
     auto go = [&](auto* index) {
-      using I = std::remove_pointer_t<decltype(index)>;
-      if (vec)
-        embedding_lookup_kernel<T, I, N><<<(unsigned)blocks, kThreads, 0, st>>>((const T*)table, rows, table_stride, index, pieces, per_row,
-                                                                              scale, (T*)out, out_stride);
-      else
-        embedding_lookup_kernel<T, I, 1><<<(unsigned)blocks, kThreads, 0, st>>>((const T*)table, rows, table_stride, index, pieces, per_row,
-                                                                              scale, (T*)out, out_stride);
+      using I = std::remove_const_t<std::remove_pointer_t<decltype(index)>>;
+      auto* kernel = piece == 2 * N ? embedding_lookup_kernel<T, I, 2 * N> : piece == N ? embedding_lookup_kernel<T, I, N> : embedding_lookup_kernel<T, I, 1>;
+      kernel<<<(unsigned)blocks, kThreads, 0, st>>>((const T*)table, rows, table_stride, index, n, per_row, kThreads / per_row, kThreads % per_row, scale,
+                                                    (T*)out, out_stride);
     };
     if (index_bits == 64) go((const int64_t*)indices);
     else go((const int32_t*)indices);
@@ -596,7 +801,7 @@ extern "C" int gnr_embedding_grad(const void* grad, int grad_type, int dim, int6
                                   int64_t rows, int64_t padding_row, float scale, int accumulate, void* out, int out_type, int64_t out_stride,
                                   void* workspace, size_t workspace_bytes, void* stream) {
   if (int rc = check_rows("gnr_embedding_grad", grad_type, rows, dim, index_bits, n)) return rc;
-  if (gnr_type_size(out_type) == 0 || !out || out_stride < dim || (n > 0 && (!grad || !indices || !workspace || grad_stride < dim))) {
+  if (gnr_type_size(out_type) == 0 || !out || out_stride < dim || (n > 0 && (!grad || !indices || grad_stride < dim))) {
     gnr_set_error("gnr_embedding_grad: null pointer, unknown type, or rows closer than %d values", dim);
     return -1;
   }
@@ -605,47 +810,61 @@ extern "C" int gnr_embedding_grad(const void* grad, int grad_type, int dim, int6
   const bool vec = dim % wide == 0 && aligned(grad, grad_stride, gnr_type_size(grad_type), 16) &&
                    aligned(out, out_stride, gnr_type_size(out_type), out_wide);
   const GradPlan p = grad_plan(n, rows, dim, vec ? wide : 1);
-  if (n > 0 && (p.total > workspace_bytes || (uintptr_t)workspace % 16 != 0)) {
+  if (p.total > 0 && (!workspace || p.total > workspace_bytes || (uintptr_t)workspace % 16 != 0)) {
     gnr_set_error("gnr_embedding_grad: workspace of %zu bytes, %zu are needed on a 16-byte boundary", workspace_bytes, p.total);
     return -1;
   }
+  // a block that fills writes up to 64 KB
+  const int64_t fill = accumulate ? 0 : std::max<int64_t>(1, std::min<int64_t>(kFillRows, 65536 / ((int64_t)dim * gnr_type_size(out_type))));
+  const int64_t blocks = p.n_blocks * p.n_cols + (accumulate ? 0 : (rows + fill - 1) / fill);
+  if (blocks > 0x7fffffff) {
+    gnr_set_error("gnr_embedding_grad: %lld tokens of %d values are too many for one call", (long long)n, dim);
+    return -1;
+  }
+  if (blocks == 0) return 0;
   char* ws = (char*)workspace;
   auto u32 = [&](size_t at) { return (uint32_t*)(ws + at); };
+  const Tokens tokens{indices, index_bits == 64, n, rows, padding_row};
   int cur = 0;
-  auto sort = [&](auto* index) {
-    using I = std::remove_const_t<std::remove_pointer_t<decltype(index)>>;
-    if (n <= kTile) {
-      const size_t smem = sizeof(SortShared) + 2 * kTile * 4;
-      GNR_CUDA_OK(cudaFuncSetAttribute(embedding_sort_block_kernel<I>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-      embedding_sort_block_kernel<I><<<1, kSortThreads, smem, st>>>(index, (int)n, rows, padding_row, p.passes, p.bits, u32(p.keys[0]),
-                                                                    u32(p.tokens[0]));
+  const bool local = n <= kLocal;
+  if (!local && n <= kClusterSort) {
+    constexpr int kEach = kClusterSort / kClusterItems;
+    auto go = [&](auto items) {
+      constexpr int Items = decltype(items)::value;
+      GNR_CUDA_OK(cudaFuncSetAttribute(embedding_sort_cluster_kernel<Items>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(ClusterShared<Items>)));
+      embedding_sort_cluster_kernel<Items><<<kCluster, kClusterWarps * 32, sizeof(ClusterShared<Items>), st>>>(tokens, p.passes, p.bits, u32(p.keys[0]),
+                                                                                                            u32(p.places[0]));
       GNR_CUDA_OK(cudaGetLastError());
       return 0;
-    }
+    };
+    if (int rc = n <= kEach       ? go(std::integral_constant<int, 1>())
+                 : n <= 2 * kEach ? go(std::integral_constant<int, 2>())
+                 : n <= 4 * kEach ? go(std::integral_constant<int, 4>())
+                                  : go(std::integral_constant<int, 8>()))
+      return rc;
+  } else if (!local) {
     for (int pass = 0; pass < p.passes; ++pass) {
-      const I* source = pass == 0 ? index : nullptr;
+      const uint32_t* keys = pass == 0 ? nullptr : u32(p.keys[cur]);
       const int shift = pass * p.bits, to = pass == 0 ? 0 : cur ^ 1;
-      GNR_CUDA_OK((cudaError_t)gnr_launch(embedding_count_kernel<I>, p.n_tiles, kSortThreads, 0, st, pass > 0, source, u32(p.keys[cur]), n, rows,
-                                          padding_row, shift, p.bits, u32(p.counts), p.n_tiles));
+      GNR_CUDA_OK((cudaError_t)gnr_launch(embedding_count_kernel, p.n_tiles, kTileWarps * 32, 0, st, pass > 0, tokens, keys, shift, p.bits,
+                                          u32(p.counts), p.n_tiles));
       GNR_CUDA_OK((cudaError_t)gnr_launch(embedding_scan_kernel, 1u << p.bits, kThreads, 0, st, true, u32(p.counts), p.n_tiles, u32(p.totals)));
-      GNR_CUDA_OK((cudaError_t)gnr_launch(embedding_scatter_kernel<I>, p.n_tiles, kSortThreads, 0, st, true, source, u32(p.keys[cur]),
-                                          u32(p.tokens[cur]), n, rows, padding_row, shift, p.bits, u32(p.counts), u32(p.totals), p.n_tiles,
-                                          u32(p.keys[to]), u32(p.tokens[to])));
+      GNR_CUDA_OK((cudaError_t)gnr_launch(embedding_scatter_kernel, p.n_tiles, kTileWarps * 32, 0, st, true, tokens, keys, u32(p.places[cur]), shift,
+                                          p.bits, u32(p.counts), u32(p.totals), p.n_tiles, u32(p.keys[to]), u32(p.places[to])));
       cur = to;
     }
-    return 0;
-  };
-  if (n > 0)
-    if (int rc = index_bits == 64 ? sort((const int64_t*)indices) : sort((const int32_t*)indices)) return rc;
+  }
   SumArgs a{};
+  a.tokens = tokens;
+  a.local = local;
+  a.passes = p.passes;
+  a.bits = p.bits;
+  a.keys = u32(p.keys[cur]);
+  a.places = u32(p.places[cur]);
   a.grad = grad;
   a.grad_stride = grad_stride;
   a.out = out;
   a.out_stride = out_stride;
-  a.keys = u32(p.keys[cur]);
-  a.tokens = u32(p.tokens[cur]);
-  a.n = n;
-  a.rows = rows;
   a.dim = dim;
   a.lanes = p.lanes;
   a.n_cols = p.n_cols;
@@ -653,28 +872,21 @@ extern "C" int gnr_embedding_grad(const void* grad, int grad_type, int dim, int6
   a.share = p.share;
   a.n_blocks = p.n_blocks;
   a.pieces = (float*)(ws + p.pieces);
+  a.keys_of = u32(p.keys_of);
   a.piece_stride = p.piece_stride;
   a.scale = scale;
-  a.accumulate = accumulate != 0;
-  // a block of the fill writes some 32 KB
-  a.fill_rows = accumulate ? 0 : std::max<int64_t>(1, std::min<int64_t>(kThreads, 32768 / ((int64_t)dim * gnr_type_size(out_type))));
-  const int64_t fill_blocks = accumulate ? 0 : (rows + a.fill_rows - 1) / a.fill_rows;
-  const int64_t blocks = p.n_blocks * p.n_cols + fill_blocks;
-  if (blocks > 0x7fffffff) {
-    gnr_set_error("gnr_embedding_grad: %lld tokens of %d values are too many for one call", (long long)n, dim);
-    return -1;
-  }
-  if (blocks == 0) return 0;
+  a.fill_rows = (int)fill;
   return gnr_with_type(grad_type, [&](auto ti) {
     return gnr_with_type(out_type, [&](auto to) {
       using TI = decltype(ti);
       using TO = decltype(to);
       constexpr int N = 16 / sizeof(TI);
-      GNR_CUDA_OK((cudaError_t)(vec ? gnr_launch(embedding_sum_kernel<TI, TO, N>, (unsigned)blocks, kThreads, 0, st, n > 0, a)
-                                    : gnr_launch(embedding_sum_kernel<TI, TO, 1>, (unsigned)blocks, kThreads, 0, st, n > 0, a)));
-      if (p.n_blocks > 1)
-        GNR_CUDA_OK((cudaError_t)(vec ? gnr_launch(embedding_join_kernel<TO, N>, (unsigned)(p.n_blocks * p.n_cols), kThreads, 0, st, true, a)
-                                      : gnr_launch(embedding_join_kernel<TO, 1>, (unsigned)(p.n_blocks * p.n_cols), kThreads, 0, st, true, a)));
+      auto* sum = vec ? accumulate ? embedding_sum_kernel<TI, TO, N, true> : embedding_sum_kernel<TI, TO, N, false>
+                      : accumulate ? embedding_sum_kernel<TI, TO, 1, true> : embedding_sum_kernel<TI, TO, 1, false>;
+      auto* join = vec ? accumulate ? embedding_join_kernel<TO, N, true> : embedding_join_kernel<TO, N, false>
+                       : accumulate ? embedding_join_kernel<TO, 1, true> : embedding_join_kernel<TO, 1, false>;
+      GNR_CUDA_OK((cudaError_t)gnr_launch(sum, (unsigned)blocks, kThreads, 0, st, !local, a));
+      if (p.n_blocks > 1) GNR_CUDA_OK((cudaError_t)gnr_launch(join, (unsigned)(p.n_blocks * p.n_cols), kThreads, 0, st, true, a));
       return 0;
     });
   });

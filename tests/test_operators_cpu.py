@@ -29,7 +29,8 @@ def test_c_entries_refuse():
 
     lib, p = _lib.lib, C.c_void_p(256)
     n = C.c_size_t(0)
-    assert lib.gnr_embedding_grad_workspace_bytes(1000, 11500, 48, C.byref(n)) == 0 and n.value >= 16000
+    assert lib.gnr_embedding_grad_workspace_bytes(100, 11500, 48, C.byref(n)) == 0 and n.value == 0  # small: in shared memory
+    assert lib.gnr_embedding_grad_workspace_bytes(100000, 11500, 48, C.byref(n)) == 0 and n.value >= 1600000
     for t, v, d in ((-1, 5, 4), (2 ** 31, 5, 4), (3, 0, 4), (3, 2 ** 31 - 1, 4), (3, 5, 0)):
         assert lib.gnr_embedding_grad_workspace_bytes(t, v, d, C.byref(n)) < 0
         assert lib.gnr_embedding_lookup(p, 0, v, d, d, p, 64, t, 1.0, p, d, None) < 0
@@ -39,11 +40,12 @@ def test_c_entries_refuse():
     assert lib.gnr_embedding_lookup(p, 0, 5, 4, 3, p, 64, 3, 1.0, p, 4, None) < 0  # rows that overlap
     assert lib.gnr_embedding_lookup(None, 0, 5, 4, 4, p, 64, 3, 1.0, p, 4, None) < 0
     assert lib.gnr_embedding_lookup(None, 0, 5, 4, 4, None, 64, 0, 1.0, None, 4, None) == 0  # nothing to do
-    assert lib.gnr_embedding_grad(p, 0, 4, 4, p, 64, 3, 5, -1, 1.0, 0, p, 0, 4, p, 16, None) < 0 and b"workspace" in lib.gnr_last_error()
+    assert lib.gnr_embedding_grad(p, 0, 4, 4, p, 64, 2000, 5, -1, 1.0, 0, p, 0, 4, p, 16, None) < 0 and b"workspace" in lib.gnr_last_error()
     assert lib.gnr_embedding_grad(p, 0, 4, 4, p, 64, 3, 5, -1, 1.0, 0, p, 0, 3, p, 1 << 30, None) < 0
     assert lib.gnr_embedding_grad(p, 0, 4, 4, p, 64, 3, 5, -1, 1.0, 0, p, 7, 4, p, 1 << 30, None) < 0
     assert lib.gnr_embedding_grad(p, 0, 4, 4, None, 64, 3, 5, -1, 1.0, 0, p, 0, 4, p, 1 << 30, None) < 0
-    assert lib.gnr_embedding_grad(p, 0, 4, 4, p, 64, 3, 5, -1, 1.0, 0, p, 0, 4, C.c_void_p(264), 1 << 30, None) < 0  # not on 16 bytes
+    assert lib.gnr_embedding_grad(p, 0, 4, 4, p, 64, 2000, 5, -1, 1.0, 0, p, 0, 4, None, 1 << 30, None) < 0
+    assert lib.gnr_embedding_grad(p, 0, 4, 4, p, 64, 2000, 5, -1, 1.0, 0, p, 0, 4, C.c_void_p(264), 1 << 30, None) < 0  # not on 16 bytes
 
 
 def test_adamw_entry_refuses():
