@@ -47,11 +47,9 @@ embedding_lookup_kernel(const T* __restrict__ table, int64_t rows, int64_t table
   for (int k = 0; k < kPieces; ++k) {
     row[k] = t < n ? (int64_t)index[t] : -1;
     to[k] = t < n ? out + t * out_stride + (int64_t)c * N : nullptr;
-    if (row[k] >= 0 && row[k] < rows) {
-      const T* from = table + row[k] * table_stride + (int64_t)c * N;
-      if constexpr (sizeof(T) * N == 32) load32(x[k], from);
-      else x[k].load(from);
-    }
+    const T* from = table + (row[k] >= 0 && row[k] < rows ? row[k] : 0) * table_stride + (int64_t)c * N;  // a row of the table in any case
+    if constexpr (sizeof(T) * N == 32) load32(x[k], from);
+    else x[k].load(from);
     t += hop_rows;
     c += hop_pieces;
     if (c >= per_row) {

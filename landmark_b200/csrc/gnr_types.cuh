@@ -53,7 +53,7 @@ template <typename T, int N, bool Words = (sizeof(T) * N >= 4)> struct Raw {
 // 32 bytes on a 32-byte boundary in one access; load32 of memory that the kernel does not write
 template <typename T, int N> __device__ __forceinline__ void load32(Raw<T, N>& x, const T* at) {
   static_assert(sizeof(x.w) == 32);
-  asm("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+  asm volatile("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
       : "=r"(x.w[0]), "=r"(x.w[1]), "=r"(x.w[2]), "=r"(x.w[3]), "=r"(x.w[4]), "=r"(x.w[5]), "=r"(x.w[6]), "=r"(x.w[7])
       : "l"(at));
 }
