@@ -13,7 +13,7 @@
 //
 // Three ways to sort, by the number of tokens: up to 1024, every block that sums sorts all of them itself (one launch for
 // the whole gradient where one block can sum them); up to 65536, a cluster of eight blocks sorts in its shared memory; above, tiles of
-// 4096 tokens are counted, scanned and scattered digit by digit.
+// 2048 tokens are counted, scanned and scattered digit by digit.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -298,7 +298,7 @@ embedding_sort_cluster_kernel(Tokens tokens, int passes, int bits, uint32_t* __r
 }
 
 constexpr int kTileWarps = 16;
-constexpr int kItems = 8;
+constexpr int kItems = 4;
 constexpr int kTile = kTileWarps * 32 * kItems;  // tokens of a tile
 
 // keys of a tile; `sorted` null: from the indices
@@ -406,6 +406,7 @@ struct SumArgs {
   void* out;
   int64_t out_stride;
   int dim, lanes, n_cols;  // lanes: pieces of a row that a block's worker takes, n_cols such parts make a row
+  int hop;                 // pieces of a row
   int workers;             // workers of a block
   int share;               // sorted tokens of a worker
   int64_t n_blocks;        // blocks along the tokens
@@ -418,26 +419,53 @@ struct SumArgs {
   int fill_rows;           // rows of a block that fills rows without a token with zeros, 0: there are none
 };
 
-template <typename TO, int N> __device__ __forceinline__ TO* row_at(const SumArgs& a, uint32_t row, int64_t c) {
-  return static_cast<TO*>(a.out) + (int64_t)row * a.out_stride + c;
-}
-
-// scale * x, added to what was there with Add
-template <typename TO, int N, bool Add> __device__ __forceinline__ void write_row(const SumArgs& a, TO* at, const float (&x)[N], const Raw<TO, N>& old) {
-  Pack<TO, N> y;
+// A piece of a row, as it is loaded and written: N neighbours from c on (Whole), or, where their alignment forbids that, the values at
+// c, c + hop, c + 2 hop ... that lie in the row, so that neighbouring threads have neighbouring values.
+template <typename T, int N, bool Whole> struct Piece {
+  std::conditional_t<Whole, Raw<T, N>, T[N]> x;
+  __device__ __forceinline__ void load(const SumArgs& a, const T* row, int64_t c) {
+    if constexpr (Whole) {
+      x.load(row + c);
+    } else {
 #pragma unroll
-  for (int k = 0; k < N; ++k) y.v[k] = from_float<TO>(Add ? fmaf(x[k], a.scale, old.get(k)) : x[k] * a.scale);
-  *reinterpret_cast<Pack<TO, N>*>(at) = y;
+      for (int k = 0; k < N; ++k) x[k] = c + k * a.hop < a.dim ? row[c + k * a.hop] : from_float<T>(0.0f);
+    }
+  }
+  __device__ __forceinline__ float get(int k) const {
+    if constexpr (Whole) return x.get(k);
+    else return to_float(x[k]);
+  }
+};
+
+// row = scale * sum, added to what was there (`old`) with Add
+template <typename T, int N, bool Whole, bool Add>
+__device__ __forceinline__ void write_row(const SumArgs& a, uint32_t row, int64_t c, const float (&sum)[N], const Piece<T, N, Whole>& old) {
+  T* at = static_cast<T*>(a.out) + (int64_t)row * a.out_stride + c;
+  T y[N];
+#pragma unroll
+  for (int k = 0; k < N; ++k) y[k] = from_float<T>(Add ? fmaf(sum[k], a.scale, old.get(k)) : sum[k] * a.scale);
+  if constexpr (Whole) {
+    Pack<T, N> z;
+#pragma unroll
+    for (int k = 0; k < N; ++k) z.v[k] = y[k];
+    *reinterpret_cast<Pack<T, N>*>(at) = z;
+  } else {
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+      if (c + k * a.hop < a.dim) at[k * a.hop] = y[k];
+  }
 }
-template <typename TO, int N, bool Add> __device__ __forceinline__ void write_row(const SumArgs& a, uint32_t row, int64_t c, const float (&x)[N]) {
-  TO* at = row_at<TO, N>(a, row, c);
-  Raw<TO, N> old{};
-  if (Add) old.load(at);
-  write_row<TO, N, Add>(a, at, x, old);
+template <typename T> __device__ __forceinline__ T* row_at(const SumArgs& a, uint32_t row) { return static_cast<T*>(a.out) + (int64_t)row * a.out_stride; }
+template <typename T, int N, bool Whole, bool Add>
+__device__ __forceinline__ void write_row(const SumArgs& a, uint32_t row, int64_t c, const float (&sum)[N]) {
+  Piece<T, N, Whole> old;
+  if (Add) old.load(a, row_at<T>(a, row), c);
+  write_row<T, N, Whole, Add>(a, row, c, sum, old);
 }
 
-__device__ __forceinline__ float* piece_at(const SumArgs& a, int64_t block, int which, int64_t c) {
-  return a.pieces + (block * 2 + which) * a.piece_stride + c;
+// where the pieces of rows that blocks share are kept: N values of a thread side by side
+__device__ __forceinline__ float* piece_at(const SumArgs& a, int64_t block, int which, int64_t at) {
+  return a.pieces + (block * 2 + which) * a.piece_stride + at;
 }
 
 // first position of the sorted keys that is not below `key`, found by a warp
@@ -518,9 +546,9 @@ template <int N> struct SumShared {
   int64_t range[2];
 };
 
-template <typename TI, typename TO, int N, bool Add> __global__ void __launch_bounds__(kThreads) embedding_sum_kernel(SumArgs a) {
+template <typename TI, typename TO, int N, bool Whole, bool Add> __global__ void __launch_bounds__(kThreads) embedding_sum_kernel(SumArgs a) {
   __shared__ SumShared<N> s;
-  constexpr int kBatch = Add ? 4 : 8;  // rows in flight
+  constexpr int kBatch = Add || !Whole ? 4 : 8;  // rows in flight
   griddep_wait();
   const int64_t sum_blocks = a.n_blocks * a.n_cols;
   if (blockIdx.x >= sum_blocks) {
@@ -552,10 +580,10 @@ template <typename TI, typename TO, int N, bool Add> __global__ void __launch_bo
   __syncthreads();
   const int worker = threadIdx.x / a.lanes;
   const int piece = (int)(blockIdx.x % a.n_cols) * a.lanes + (int)threadIdx.x % a.lanes;
-  const bool on = worker < a.workers && (int64_t)piece * N < a.dim;
-  const int64_t c = (int64_t)piece * N;
+  const bool on = worker < a.workers && piece < a.hop;
+  const int64_t c = Whole ? (int64_t)piece * N : piece;
   const int begin = worker * a.share, end = min(begin + a.share, s.valid);
-  const TI* grad = static_cast<const TI*>(a.grad) + c;
+  const TI* grad = static_cast<const TI*>(a.grad);
   bool through = false, tail = false;
   if (on && begin < end) {
     bool first = keys[begin - 1] == keys[begin];  // the row that began before the share
@@ -563,14 +591,14 @@ template <typename TI, typename TO, int N, bool Add> __global__ void __launch_bo
 #pragma unroll
     for (int k = 0; k < N; ++k) acc[k] = 0.0f;
     for (int i = begin; i < end; i += kBatch) {
-      Raw<TI, N> x[kBatch];
-      Raw<TO, N> old[Add ? kBatch : 1];
+      Piece<TI, N, Whole> x[kBatch];
+      Piece<TO, N, Whole> old[Add ? kBatch : 1];
 #pragma unroll
-      for (int b = 0; b < kBatch; ++b) x[b].load(grad + (int64_t)tokens[min(i + b, end - 1)] * a.grad_stride);
+      for (int b = 0; b < kBatch; ++b) x[b].load(a, grad + (int64_t)tokens[min(i + b, end - 1)] * a.grad_stride, c);
       if constexpr (Add) {
 #pragma unroll
         for (int b = 0; b < kBatch; ++b)
-          if (i + b < end && keys[i + b + 1] != keys[i + b]) old[b].load(row_at<TO, N>(a, keys[i + b], c));
+          if (i + b < end && keys[i + b + 1] != keys[i + b]) old[b].load(a, row_at<TO>(a, keys[i + b]), c);
       }
 #pragma unroll
       for (int b = 0; b < kBatch; ++b) {
@@ -583,7 +611,7 @@ template <typename TI, typename TO, int N, bool Add> __global__ void __launch_bo
 #pragma unroll
             for (int k = 0; k < N; ++k) s.head[threadIdx.x][k] = acc[k];
           } else {
-            write_row<TO, N, Add>(a, row_at<TO, N>(a, key, c), acc, old[Add ? b : 0]);
+            write_row<TO, N, Whole, Add>(a, key, c, acc, old[Add ? b : 0]);
           }
           first = false;
 #pragma unroll
@@ -623,9 +651,9 @@ template <typename TI, typename TO, int N, bool Add> __global__ void __launch_bo
       open = s.through[t];
     }
     if (kind == 1 && !open) {
-      write_row<TO, N, Add>(a, keys[end - 1], c, acc);
+      write_row<TO, N, Whole, Add>(a, keys[end - 1], c, acc);
     } else {
-      float* at = piece_at(a, block, kind, c);
+      float* at = piece_at(a, block, kind, (int64_t)piece * N);
 #pragma unroll
       for (int k = 0; k < N; ++k) at[k] = acc[k];
     }
@@ -633,7 +661,7 @@ template <typename TI, typename TO, int N, bool Add> __global__ void __launch_bo
 }
 
 // Rows that several blocks share: the block that one begins in adds the others' pieces, its workers equal shares of them.
-template <typename TO, int N, bool Add> __global__ void __launch_bounds__(kThreads) embedding_join_kernel(SumArgs a) {
+template <typename TO, int N, bool Whole, bool Add> __global__ void __launch_bounds__(kThreads) embedding_join_kernel(SumArgs a) {
   __shared__ float s_sum[kThreads][N];
   griddep_wait();
   const int64_t block = blockIdx.x / a.n_cols;
@@ -648,17 +676,17 @@ template <typename TO, int N, bool Add> __global__ void __launch_bounds__(kThrea
   }
   const int worker = threadIdx.x / a.lanes;
   const int piece = (int)(blockIdx.x % a.n_cols) * a.lanes + (int)threadIdx.x % a.lanes;
-  const bool on = worker < a.workers && (int64_t)piece * N < a.dim;
-  const int64_t c = (int64_t)piece * N;
+  const bool on = worker < a.workers && piece < a.hop;
+  const int64_t c = Whole ? (int64_t)piece * N : piece;
   const int64_t each = (count + a.workers - 1) / a.workers;
   const int64_t from = block + 1 + min(worker * each, count), to = block + 1 + min((worker + 1) * each, count);
   float acc[N];
 #pragma unroll
-  for (int k = 0; k < N; ++k) acc[k] = on && worker == 0 ? piece_at(a, block, 1, c)[k] : 0.0f;
+  for (int k = 0; k < N; ++k) acc[k] = on && worker == 0 ? piece_at(a, block, 1, (int64_t)piece * N)[k] : 0.0f;
   if (on) {
 #pragma unroll 8
     for (int64_t b = from; b < to; ++b) {
-      const float* at = piece_at(a, b, 0, c);
+      const float* at = piece_at(a, b, 0, (int64_t)piece * N);
 #pragma unroll
       for (int k = 0; k < N; ++k) acc[k] += at[k];
     }
@@ -670,7 +698,7 @@ template <typename TO, int N, bool Add> __global__ void __launch_bounds__(kThrea
   for (int w = 1; w < a.workers && w * each < count; ++w)
 #pragma unroll
     for (int k = 0; k < N; ++k) acc[k] += s_sum[w * a.lanes + threadIdx.x][k];
-  write_row<TO, N, Add>(a, key, c, acc);
+  write_row<TO, N, Whole, Add>(a, key, c, acc);
 }
 
 // ---- plan ----------------------------------------------------------------------------------------------------------
@@ -679,7 +707,7 @@ size_t align256(size_t v) { return (v + 255) / 256 * 256; }
 
 // Everything that the sizes decide.
 struct GradPlan {
-  int lanes, n_cols, workers, share;
+  int hop, lanes, n_cols, workers, share;
   int64_t n_blocks, piece_stride;
   int passes, bits, n_tiles;
   size_t keys[2], places[2], counts, totals, pieces, keys_of, total;
@@ -688,8 +716,9 @@ struct GradPlan {
 GradPlan grad_plan(int64_t n, int64_t rows, int dim, int n_values) {
   GradPlan p{};
   const int per_row = (dim + n_values - 1) / n_values;
-  p.lanes = std::min(per_row, kThreads);
-  p.n_cols = (per_row + p.lanes - 1) / p.lanes;
+  p.hop = per_row;
+  p.n_cols = (per_row + kThreads - 1) / kThreads;
+  p.lanes = (per_row + p.n_cols - 1) / p.n_cols;
   p.workers = kThreads / p.lanes;
   // as many tokens to a worker as let two waves of half-full SMs cover them; one block where that is not far off
   const int64_t wave = (int64_t)GNR_SM_COUNT_FALLBACK * 2048;
@@ -790,7 +819,7 @@ extern "C" int gnr_embedding_grad_workspace_bytes(int64_t n, int64_t rows, int d
     return -1;
   }
   size_t most = 0;  // of the layouts that the alignments may choose
-  for (int n_values : {1, 4, 8}) most = std::max(most, grad_plan(n, rows, dim, n_values).total);
+  for (int n_values : {4, 8}) most = std::max(most, grad_plan(n, rows, dim, n_values).total);
   *bytes_h = most;
   return 0;
 }
@@ -807,13 +836,14 @@ extern "C" int gnr_embedding_grad(const void* grad, int grad_type, int dim, int6
   const int wide = 16 / gnr_type_size(grad_type), out_wide = std::min(16, wide * gnr_type_size(out_type));
   const bool vec = dim % wide == 0 && aligned(grad, grad_stride, gnr_type_size(grad_type), 16) &&
                    aligned(out, out_stride, gnr_type_size(out_type), out_wide);
-  const GradPlan p = grad_plan(n, rows, dim, vec ? wide : 1);
+  const GradPlan p = grad_plan(n, rows, dim, vec ? wide : 4);
   if (p.total > 0 && (!workspace || p.total > workspace_bytes || (uintptr_t)workspace % 16 != 0)) {
     gnr_set_error("gnr_embedding_grad: workspace of %zu bytes, %zu are needed on a 16-byte boundary", workspace_bytes, p.total);
     return -1;
   }
-  // a block that fills writes up to 64 KB
-  const int64_t fill = accumulate ? 0 : std::max<int64_t>(1, std::min<int64_t>(kFillRows, 65536 / ((int64_t)dim * gnr_type_size(out_type))));
+  // blocks that fill: three to an SM, with 16 KB to write at least and kFillRows rows at most
+  const int64_t fill = accumulate ? 0 : std::min<int64_t>(kFillRows, std::max<int64_t>((rows + 3 * GNR_SM_COUNT_FALLBACK - 1) / (3 * GNR_SM_COUNT_FALLBACK),
+                                                                                16384 / ((int64_t)dim * gnr_type_size(out_type)) + 1));
   const int64_t blocks = p.n_blocks * p.n_cols + (accumulate ? 0 : (rows + fill - 1) / fill);
   if (blocks > 0x7fffffff) {
     gnr_set_error("gnr_embedding_grad: %lld tokens of %d values are too many for one call", (long long)n, dim);
@@ -864,6 +894,7 @@ extern "C" int gnr_embedding_grad(const void* grad, int grad_type, int dim, int6
   a.out = out;
   a.out_stride = out_stride;
   a.dim = dim;
+  a.hop = p.hop;
   a.lanes = p.lanes;
   a.n_cols = p.n_cols;
   a.workers = p.workers;
@@ -879,10 +910,10 @@ extern "C" int gnr_embedding_grad(const void* grad, int grad_type, int dim, int6
       using TI = decltype(ti);
       using TO = decltype(to);
       constexpr int N = 16 / sizeof(TI);
-      auto* sum = vec ? accumulate ? embedding_sum_kernel<TI, TO, N, true> : embedding_sum_kernel<TI, TO, N, false>
-                      : accumulate ? embedding_sum_kernel<TI, TO, 1, true> : embedding_sum_kernel<TI, TO, 1, false>;
-      auto* join = vec ? accumulate ? embedding_join_kernel<TO, N, true> : embedding_join_kernel<TO, N, false>
-                       : accumulate ? embedding_join_kernel<TO, 1, true> : embedding_join_kernel<TO, 1, false>;
+      auto* sum = vec ? accumulate ? embedding_sum_kernel<TI, TO, N, true, true> : embedding_sum_kernel<TI, TO, N, true, false>
+                      : accumulate ? embedding_sum_kernel<TI, TO, 4, false, true> : embedding_sum_kernel<TI, TO, 4, false, false>;
+      auto* join = vec ? accumulate ? embedding_join_kernel<TO, N, true, true> : embedding_join_kernel<TO, N, true, false>
+                       : accumulate ? embedding_join_kernel<TO, 4, false, true> : embedding_join_kernel<TO, 4, false, false>;
       GNR_CUDA_OK((cudaError_t)gnr_launch(sum, (unsigned)blocks, kThreads, 0, st, !local, a));
       if (p.n_blocks > 1) GNR_CUDA_OK((cudaError_t)gnr_launch(join, (unsigned)(p.n_blocks * p.n_cols), kThreads, 0, st, true, a));
       return 0;
