@@ -171,14 +171,16 @@ class AdamW(torch.optim.Optimizer):
         self._sets.clear()
 
     def load_state_dict(self, state_dict):
-        """Restores what ``state_dict`` returned, every state in its own type (torch would give it the parameter's)."""
+        """Restores what ``state_dict`` returned, every state in its own type (torch would give it the parameter's).  The state of a
+        ``torch.optim.AdamW`` with fp32 moments is taken as well."""
         super().load_state_dict(state_dict)
         self._sets.clear()
         saved = state_dict["state"]
         ids = [i for group in state_dict["param_groups"] for i in group["params"]]
         for i, p in zip(ids, [p for group in self.param_groups for p in group["params"]]):
             if i in saved:
-                self.state[p] = {k: v.detach().to(p.device, copy=True) if isinstance(v, torch.Tensor) else v for k, v in saved[i].items()}
+                self.state[p] = {k: int(v) if k == "step" else v.detach().to(p.device, copy=True) if isinstance(v, torch.Tensor) else v
+                                 for k, v in saved[i].items()}
 
     def __getstate__(self):
         return {**super().__getstate__(), "state_bits": self.state_bits, "master_weights": self.master_weights, "seed": self.seed}
@@ -197,8 +199,8 @@ class AdamW(torch.optim.Optimizer):
                 if self.state_bits == 8:
                     s[name] = s[name].view(kind)
                     s[name + "_scale"] = torch.zeros(state_blocks(p.numel()), device=p.device)
-            if self.master_weights and p.dtype != torch.float32:
-                s["master"] = p.detach().float()
+        if self.master_weights and p.dtype != torch.float32 and "master" not in s:
+            s["master"] = p.detach().float()
         return s
 
     def _tensors(self, key, params) -> Tuple[list, AdamWTensors]:

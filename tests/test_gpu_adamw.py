@@ -288,6 +288,65 @@ def test_optimiser_state_survives(state_bits):
     assert all(torch.equal(x, y) for x, y in zip(a, b))
 
 
+def test_state_of_torch_adamw_is_taken():
+    """Five steps of torch's AdamW, then five of this one with its state, against ten in 64 bits (tolerance as above, torch's step rounds no
+    more often)."""
+    from landmark_b200.optim import AdamW
+
+    torch.manual_seed(3)
+    p = [torch.nn.Parameter(torch.randn(n, device="cuda")) for n in (700, 33)]
+    x, m, v = ([f(t.detach().double()) for t in p] for f in (torch.clone, torch.zeros_like, torch.zeros_like))
+    opt = torch.optim.AdamW(p, lr=1e-2, weight_decay=0.1)
+    for t in range(10):
+        if t == 5:
+            mine = AdamW(p, lr=1e-2, weight_decay=0.1)
+            mine.load_state_dict(opt.state_dict())
+            opt = mine
+        for k in range(2):
+            p[k].grad = torch.randn_like(p[k])
+            (x[k], m[k], v[k]), _ = reference(x[k], p[k].grad.double(), m[k], v[k], t + 1, 1e-2, (0.9, 0.999), 1e-8, 0.1)
+        opt.step()
+    for k in range(2):
+        assert bool(((p[k].double() - x[k]).abs() <= 10 * 20 * U * (x[k].abs() + 1)).all())
+
+
+@pytest.mark.parametrize("state_bits", [8, 32])
+def test_copied_and_saved_optimisers_go_on(state_bits):
+    import io
+    import pickle
+
+    from landmark_b200.optim import AdamW
+
+    p = torch.nn.Parameter(torch.randn(600, device="cuda"))
+    opt = AdamW([p], lr=1e-2, state_bits=state_bits, seed=4)
+    g = torch.randn(600, device="cuda")
+    p.grad = g.clone()
+    opt.step()
+
+    def saved_and_loaded():
+        file = io.BytesIO()
+        torch.save(opt.state_dict(), file)
+        file.seek(0)
+        new = AdamW([torch.nn.Parameter(p.detach().clone())], lr=1e-2, state_bits=state_bits, seed=4)
+        new.load_state_dict(torch.load(file))
+        return new
+
+    ways = [lambda: copy.deepcopy(opt), saved_and_loaded]
+    if state_bits == 32:  # (torch cannot pickle float8 tensors outside torch.save)
+        ways.append(lambda: pickle.loads(pickle.dumps(opt)))
+    for way in ways:
+        again = way()
+        assert (again.state_bits, again.seed, again.master_weights) == (state_bits, 4, True)
+        q = again.param_groups[0]["params"][0]
+        kept = p.detach().clone(), copy.deepcopy(opt.state_dict())
+        q.grad = g.clone()
+        again.step()
+        opt.step()
+        assert torch.equal(p, q) and q.data_ptr() != p.data_ptr()
+        p.data.copy_(kept[0])
+        opt.load_state_dict(kept[1])
+
+
 def test_memory_that_moved_and_captures_are_refused():
     from landmark_b200.optim import AdamWTensors
 

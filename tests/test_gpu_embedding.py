@@ -130,6 +130,35 @@ def test_gradient(dtype, t, v, d, spread):
     assert torch.equal(got, embedding_backward(g, idx.to(torch.int32), v))  # and the same bits again
 
 
+# where the way of sorting, the number of blocks or the number of passes changes, and one beside it
+BORDERS = [(n + k, v, d) for n, v, d in ((672, 11500, 48), (1024, 11500, 48), (8192, 511, 4), (16384, 512, 4), (32768, 262143, 4), (65536, 262144, 4),
+                                         (2048 * 40, 3, 1)) for k in (0, 1)]
+
+
+@pytest.mark.parametrize("t,v,d", BORDERS)
+@pytest.mark.parametrize("spread", ["uniform", "runs", "one"])
+def test_gradient_at_borders(t, v, d, spread):
+    from landmark_b200.embedding import embedding_backward
+
+    idx, g, _ = make(t, v, d, torch.float32, spread, masked=0.02, seed=1)
+    idx[:: max(1, t // 7)] = v - 1  # the last row is named
+    got = embedding_backward(g, idx, v)
+    check_gradient(got, g, idx, v)
+    assert torch.equal(got, embedding_backward(g, idx, v))
+
+
+@pytest.mark.parametrize("d", [1, 2, 3, 5, 255, 257, 1023, 1025, 4100])
+def test_gradient_of_odd_widths(d):
+    from landmark_b200.embedding import embedding_backward
+
+    for dtype, out in ((torch.float32, torch.float32), (torch.bfloat16, torch.float32), (torch.float16, torch.float16)):
+        for t in (700, 3000):
+            idx, g, _ = make(t, 90, d, dtype, "runs", masked=0.1)
+            check_gradient(embedding_backward(g, idx, 90, dtype=out), g, idx, 90)
+            old = torch.randn((90, d), device="cuda").to(out)
+            check_gradient(embedding_backward(g, idx, 90, scale=2.0, out=old.clone(), accumulate=True), g, idx, 90, 2.0, old=old)
+
+
 @pytest.mark.parametrize("out", TYPES)
 @pytest.mark.parametrize("dtype", TYPES)
 def test_gradient_types_and_accumulation(dtype, out):
@@ -202,10 +231,11 @@ def test_gradients_of_each_other():
     assert torch.allclose(again, ref, rtol=1e-5, atol=1e-5)
 
 
-def test_streams_and_graphs():
+@pytest.mark.parametrize("t", [300, 6000, 70000])
+def test_streams_and_graphs(t):
     from landmark_b200.embedding import embedding, embedding_backward
 
-    idx, g, w = make(6000, 500, 48, torch.float32)
+    idx, g, w = make(t, 500, 48, torch.float32)
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):
@@ -219,13 +249,37 @@ def test_streams_and_graphs():
         with torch.cuda.graph(graph):
             out = embedding(idx, w, scale=k + 1.0), embedding_backward(g, idx, 500, scale=k + 1.0)
         graphs.append((graph, out))
-    idx2, g2, w2 = make(6000, 500, 48, torch.float32, "runs", masked=0.1, seed=5)
+    idx2, g2, w2 = make(t, 500, 48, torch.float32, "runs", masked=0.1, seed=5)
     idx.copy_(idx2), g.copy_(g2), w.copy_(w2)
     for graph, _ in graphs + graphs:
         graph.replay()
     torch.cuda.synchronize()
     for k, (_, (a, b)) in enumerate(graphs):
         assert torch.equal(a, embedding(idx, w, scale=k + 1.0)) and torch.equal(b, embedding_backward(g, idx, 500, scale=k + 1.0))
+
+
+def test_two_threads_at_once():
+    """Calls of host threads with streams of their own do not disturb each other."""
+    import threading
+
+    from landmark_b200.embedding import embedding, embedding_backward
+
+    jobs = [make(n, 700, 48, torch.float32, "runs", seed=n) for n in (900, 5000, 80000)]
+    want = [(embedding(i, w), embedding_backward(g, i, 700)) for i, g, w in jobs]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(k):
+        i, g, w = jobs[k]
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(30):
+                if not (torch.equal(embedding(i, w), want[k][0]) and torch.equal(embedding_backward(g, i, 700), want[k][1])):
+                    wrong.append(k)
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(3)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert not wrong
 
 
 def test_backward_pass_under_capture_is_refused():
