@@ -224,10 +224,13 @@ __device__ __forceinline__ void decode4(uint32_t codes, float (&x)[4]) {
 
 // the same four values as they lie in memory
 template <bool Wide, int Hop, typename T> __device__ __forceinline__ Pack<T, 4> load_raw(const T* at, int i, int end) {
-  if constexpr (Wide) return *reinterpret_cast<const Pack<T, 4>*>(at + i);
   Pack<T, 4> y;
+  if constexpr (Wide) {
+    y = *reinterpret_cast<const Pack<T, 4>*>(at + i);
+  } else {
 #pragma unroll
-  for (int k = 0; k < 4; ++k) y.v[k] = i + k * Hop < end ? at[i + k * Hop] : from_float<T>(0.0f);
+    for (int k = 0; k < 4; ++k) y.v[k] = i + k * Hop < end ? at[i + k * Hop] : from_float<T>(0.0f);
+  }
   return y;
 }
 template <bool Wide, int Hop> __device__ __forceinline__ uint32_t load_codes(const uint8_t* at, int i, int end) {
