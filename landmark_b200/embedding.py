@@ -24,29 +24,30 @@ _TYPES = {torch.float32: _lib.FP32, torch.float16: _lib.FP16, torch.bfloat16: _l
 _INDEX_BITS = {torch.int64: 64, torch.int32: 32}
 
 
-class _on:
-    """Device guard that costs nothing where the device is the current one."""
-
-    __slots__ = ("guard",)
-
-    def __init__(self, index: int):
-        self.guard = None if index == torch.cuda.current_device() else torch.cuda.device(index)
+class _Here:
+    """Stands for the device guard where the device is the current one."""
 
     def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
+        pass
 
     def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+        pass
+
+
+_here = _Here()
+
+
+def _on(index: int):
+    return _here if index == _current_device() else torch.cuda.device(index)
 
 
 def _raw_stream(index: int) -> int:
     return torch.cuda.current_stream(index).cuda_stream
 
 
-# the same without a Stream object in between (2 us a call), where this torch has it
+# the same without a Stream object and a look at CUDA's initialisation in between (2 us a call), where this torch has them
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _raw_stream)
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def _kind(what: str, t: torch.Tensor) -> int:
@@ -116,10 +117,10 @@ def _gradient(grad: torch.Tensor, indices: torch.Tensor, scale: float, padding_i
     indices = indices.contiguous()
     with _on(device):
         need = _workspace_need(n, rows, dim)
-        ws = torch.empty(need, dtype=torch.uint8, device=grad.device)
+        ws = torch.empty(need, dtype=torch.uint8, device=grad.device) if need else None
         check(lib.gnr_embedding_grad(grad.data_ptr(), kind, dim, stride, indices.data_ptr(), bits, n, rows,
                                      -1 if padding_idx is None else padding_idx, scale, accumulate, out.data_ptr(), _TYPES[out.dtype],
-                                     out.stride(0) if rows > 1 else dim, ws.data_ptr(), need, _raw_stream(device)), "gnr_embedding_grad")
+                                     out.stride(0) if rows > 1 else dim, ws.data_ptr() if need else None, need, _raw_stream(device)), "gnr_embedding_grad")
     return out
 
 
