@@ -27,7 +27,8 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kBlock = GNR_ADAMW_BLOCK;
 constexpr int kChunk = 4096;                       // values of a thread block
-constexpr int kChunk8 = kThreads / 32 * kBlock;    // ... with 8-bit states: a block of codes for each warp
+constexpr int kThreads8 = 256;                     // with 8-bit states
+constexpr int kChunk8 = kThreads8 / 32 * kBlock;   // ... a block of codes for each warp
 constexpr float kTop = 448.0f;
 
 struct Tensor {
@@ -124,18 +125,18 @@ __device__ __forceinline__ float stepped(const Hyper& h, float x, float m, float
   return x * h.keep - h.rate * (m * quick_rcp(root * h.c2_inv + h.eps));
 }
 
-// Four values of a thread: the neighbours from i on, or (not Wide) those Hop apart from i on that lie before `end`, 0 for the others.
-template <bool Wide, int Hop, typename T> __device__ __forceinline__ void load4(const T* at, int i, int end, float (&x)[4]) {
+// Four values of a thread: the neighbours from i on, or (not Wide) those kThreads apart from i on that lie before `end`, 0 for the others.
+template <bool Wide, typename T> __device__ __forceinline__ void load4(const T* at, int i, int end, float (&x)[4]) {
   if constexpr (Wide) {
     const Pack<T, 4> y = *reinterpret_cast<const Pack<T, 4>*>(at + i);
 #pragma unroll
     for (int k = 0; k < 4; ++k) x[k] = to_float(y.v[k]);
   } else {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) x[k] = i + k * Hop < end ? to_float(at[i + k * Hop]) : 0.0f;
+    for (int k = 0; k < 4; ++k) x[k] = i + k * kThreads < end ? to_float(at[i + k * kThreads]) : 0.0f;
   }
 }
-template <bool Wide, int Hop, typename T> __device__ __forceinline__ void store4(T* at, int i, int end, const float (&x)[4]) {
+template <bool Wide, typename T> __device__ __forceinline__ void store4(T* at, int i, int end, const float (&x)[4]) {
   if constexpr (Wide) {
     Pack<T, 4> y;
 #pragma unroll
@@ -144,7 +145,7 @@ template <bool Wide, int Hop, typename T> __device__ __forceinline__ void store4
   } else {
 #pragma unroll
     for (int k = 0; k < 4; ++k)
-      if (i + k * Hop < end) at[i + k * Hop] = from_float<T>(x[k]);
+      if (i + k * kThreads < end) at[i + k * kThreads] = from_float<T>(x[k]);
   }
 }
 
@@ -182,11 +183,11 @@ __global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__
 #pragma unroll
     for (int r = 0; r < kEach; ++r) {
       const int i = Wide ? (r * kThreads + threadIdx.x) * 4 : r * kThreads * 4 + threadIdx.x;
-      load4<Wide, kThreads>(g_at, i, left, g[r]);
-      load4<Wide, kThreads>(m_at, i, left, m[r]);
-      load4<Wide, kThreads>(v_at, i, left, v[r]);
-      if constexpr (Master) load4<Wide, kThreads>(master_at, i, left, x[r]);
-      else load4<Wide, kThreads>(p_at, i, left, x[r]);
+      load4<Wide>(g_at, i, left, g[r]);
+      load4<Wide>(m_at, i, left, m[r]);
+      load4<Wide>(v_at, i, left, v[r]);
+      if constexpr (Master) load4<Wide>(master_at, i, left, x[r]);
+      else load4<Wide>(p_at, i, left, x[r]);
     }
 #pragma unroll
     for (int r = 0; r < kEach; ++r) {
@@ -196,10 +197,10 @@ __global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__
         moments(h, g[r][k], m[r][k], v[r][k]);
         x[r][k] = stepped(h, x[r][k], m[r][k], sqrtf(v[r][k]));
       }
-      store4<Wide, kThreads>(m_at, i, left, m[r]);
-      store4<Wide, kThreads>(v_at, i, left, v[r]);
-      if constexpr (Master) store4<Wide, kThreads>(master_at, i, left, x[r]);
-      store4<Wide, kThreads>(p_at, i, left, x[r]);
+      store4<Wide>(m_at, i, left, m[r]);
+      store4<Wide>(v_at, i, left, v[r]);
+      if constexpr (Master) store4<Wide>(master_at, i, left, x[r]);
+      store4<Wide>(p_at, i, left, x[r]);
     }
   };
   if (left == kChunk && all_wide<P, G, Master>(t, 16)) all(std::true_type());
@@ -222,32 +223,41 @@ __device__ __forceinline__ void decode4(uint32_t codes, float (&x)[4]) {
   }
 }
 
-// the same four values as they lie in memory
-template <bool Wide, int Hop, typename T> __device__ __forceinline__ Pack<T, 4> load_raw(const T* at, int i, int end) {
-  Pack<T, 4> y;
-  if constexpr (Wide) {
-    y = *reinterpret_cast<const Pack<T, 4>*>(at + i);
-  } else {
+template <typename T> __device__ __forceinline__ void store_some(T* at, bool whole, int count, const float (&x)[4]) {
+  if (whole) {
+    Pack<T, 4> y;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) y.v[k] = i + k * Hop < end ? at[i + k * Hop] : from_float<T>(0.0f);
-  }
-  return y;
-}
-template <bool Wide, int Hop> __device__ __forceinline__ uint32_t load_codes(const uint8_t* at, int i, int end) {
-  if constexpr (Wide) return *reinterpret_cast<const uint32_t*>(at + i);
-  uint32_t codes = 0;
-#pragma unroll
-  for (int k = 0; k < 4; ++k) codes |= i + k * Hop < end ? (uint32_t)at[i + k * Hop] << (8 * k) : 0u;
-  return codes;
-}
-template <bool Wide, int Hop> __device__ __forceinline__ void store_codes(uint8_t* at, int i, int end, uint32_t codes) {
-  if constexpr (Wide) {
-    *reinterpret_cast<uint32_t*>(at + i) = codes;
+    for (int k = 0; k < 4; ++k) y.v[k] = from_float<T>(x[k]);
+    *reinterpret_cast<Pack<T, 4>*>(at) = y;
   } else {
 #pragma unroll
     for (int k = 0; k < 4; ++k)
-      if (i + k * Hop < end) at[i + k * Hop] = (uint8_t)(codes >> (8 * k));
+      if (k < count) at[k] = from_float<T>(x[k]);
   }
+}
+
+// `count` (at most 4) neighbours as they lie in memory, zeros behind them
+template <typename T> __device__ __forceinline__ Pack<T, 4> load_raw(const T* at, bool whole, int count) {
+  if (whole) return *reinterpret_cast<const Pack<T, 4>*>(at);
+  Pack<T, 4> y;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) y.v[k] = k < count ? at[k] : from_float<T>(0.0f);
+  return y;
+}
+
+__device__ __forceinline__ uint32_t load_codes(const uint8_t* at, bool whole, int count) {
+  if (whole) return *reinterpret_cast<const uint32_t*>(at);
+  uint32_t codes = 0;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) if (k < count) codes |= (uint32_t)at[k] << (8 * k);
+  return codes;
+}
+
+__device__ __forceinline__ void store_codes(uint8_t* at, bool whole, int count, uint32_t codes) {
+  if (whole) *reinterpret_cast<uint32_t*>(at) = codes;
+  else
+#pragma unroll
+    for (int k = 0; k < 4; ++k) if (k < count) at[k] = (uint8_t)(codes >> (8 * k));
 }
 
 // Codes by the bits of an fp32 number: its exponent and three mantissa bits, 960 = (127 - 7) << 3 lower, are the e4m3 code of a
@@ -296,7 +306,7 @@ __device__ __forceinline__ void codes_of_root(const float (&root)[2], Two inv, c
   }
 }
 
-// a lane's part of a block of 256 values as it lies in memory: four values of each half, neighbours (Full) or 32 apart
+// a lane's part of a block of 256 values as it lies in memory: the four values at 4 * lane and the four 128 behind them
 template <typename X, typename G> struct Part {
   Pack<X, 4> x[2];
   Pack<G, 4> g[2];
@@ -322,11 +332,7 @@ template <typename P, typename G, bool Master> struct Chunk8 {
   uint32_t place;  // low half of the first one's place in the tensor
   uint32_t seed;
 
-  // a lane's first value in half s of the block that begins at `at`
-  template <bool Full> __device__ __forceinline__ int lane_at(int at, int s) const {
-    return at + s * 128 + (Full ? 4 : 1) * (int)(threadIdx.x & 31);
-  }
-
+  // the part at `at` = 4 * lane past the beginning of a block
   template <bool Full> __device__ __forceinline__ Part<X, G> fetch(int at) const {
     Part<X, G> part;
     const X* x_at = Master ? reinterpret_cast<const X*>(master_at) : reinterpret_cast<const X*>(p_at);
@@ -334,17 +340,17 @@ template <typename P, typename G, bool Master> struct Chunk8 {
     part.v_scale = vs_at[at / kBlock];
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-      const int i = lane_at<Full>(at, s);
-      part.g[s] = load_raw<Full, 32>(g_at, i, left);
-      part.m[s] = load_codes<Full, 32>(m_at, i, left);
-      part.v[s] = load_codes<Full, 32>(v_at, i, left);
-      part.x[s] = load_raw<Full, 32>(x_at, i, left);
+      const int i = at + s * 128;
+      const int count = Full ? 4 : min(4, max(0, left - i));
+      part.g[s] = load_raw(g_at + i, Full, count);
+      part.m[s] = load_codes(m_at + i, Full, count);
+      part.v[s] = load_codes(v_at + i, Full, count);
+      part.x[s] = load_raw(x_at + i, Full, count);
     }
     return part;
   }
 
   template <bool Full> __device__ __forceinline__ void step(const Hyper& h, const Part<X, G>& part, int at) const {
-    constexpr int kApart = Full ? 1 : 32;
     float x[2][4], g[2][4], m[2][4], root[2][4];
     uint32_t m_bits = 0, v_bits = 0;
 #pragma unroll
@@ -380,9 +386,10 @@ template <typename P, typename G, bool Master> struct Chunk8 {
         m_bits = max(max(m_bits, __float_as_uint(m[s][k]) & 0x7fffffffu), __float_as_uint(m[s][k + 1]) & 0x7fffffffu);
         v_bits = max(max(v_bits, __float_as_uint(root[s][k])), __float_as_uint(root[s][k + 1]));
       }
-      const int i = lane_at<Full>(at, s);
-      if constexpr (Master) store4<Full, 32>(master_at, i, left, x[s]);
-      store4<Full, 32>(p_at, i, left, x[s]);
+      const int i = at + s * 128;
+      const int count = Full ? 4 : min(4, max(0, left - i));
+      if constexpr (Master) store_some(master_at + i, Full, count, x[s]);
+      store_some(p_at + i, Full, count, x[s]);
     }
     m_bits = __reduce_max_sync(0xffffffffu, m_bits);  // non-negative numbers are ordered as their bits are
     v_bits = __reduce_max_sync(0xffffffffu, v_bits);
@@ -406,11 +413,12 @@ template <typename P, typename G, bool Master> struct Chunk8 {
     const float m_inv = scale_up(m_top), v_inv = scale_up(v_top);
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-      const int i = lane_at<Full>(at, s);
+      const int i = at + s * 128;
+      const int count = Full ? 4 : min(4, max(0, left - i));
       uint32_t m_codes = 0, v_codes = 0;
 #pragma unroll
       for (int k = 0; k < 4; k += 2) {
-        const uint32_t r32[2] = {hash32(place + i + k * kApart, seed), hash32(place + i + (k + 1) * kApart, seed)};
+        const uint32_t r32[2] = {hash32(place + i + k, seed), hash32(place + i + k + 1, seed)};
         const float mk[2] = {m[s][k], m[s][k + 1]}, rk[2] = {root[s][k], root[s][k + 1]};
         uint32_t m_code[2], v_code[2];
         codes_of_m(mk, two(m_inv), r32, m_code);
@@ -425,8 +433,8 @@ template <typename P, typename G, bool Master> struct Chunk8 {
           if ((__float_as_uint(root[s][k]) & 0x7fffffffu) >= kNotFinite) v_codes = (v_codes & ~(0xffu << (8 * k))) | kNanCode << (8 * k);
         }
       }
-      store_codes<Full, 32>(m_at, i, left, m_codes);
-      store_codes<Full, 32>(v_at, i, left, v_codes);
+      store_codes(m_at + i, Full, count, m_codes);
+      store_codes(v_at + i, Full, count, v_codes);
     }
     if ((threadIdx.x & 31) == 0) {
       ms_at[at / kBlock] = __fmul_rn(m_top, 1.0f / kTop);
@@ -435,11 +443,13 @@ template <typename P, typename G, bool Master> struct Chunk8 {
   }
 };
 
-// A warp takes one block of 256 values.  Bound by its 89 instructions a value (packed fp32 ones count for two values) and, at 88 % of
-// the copy rate, by HBM: 335M fp32 values 948 us, 5.68 TB/s.  Five thread blocks to an SM hide the loads better than a
-// longer run of blocks with the next one's loads ahead of the work (1058 us at its best length), six spill (1000 us).
+// A warp takes one block of 256 values.  Bound by its instructions, 89 a value with the packed fp32 ones counted for two (85 % of the issue
+// slots), and by the power they draw: 335M fp32 values take 991 us at 1965 MHz, 5.4 TB/s, and 1080 to 1150 us in a long run, where the power
+// cap holds the clock at 1.65 to 1.75 GHz.  Five thread blocks to an SM hide the loads better than a longer run of blocks with the
+// next one's loads ahead of the work (1058 against 948 us on zeros), six spill (1000).  A root by Newton's step from the quick reciprocal
+// root, with a way out for its range, saves instructions and loses their overlap (1091 against 997 us).
 template <typename P, typename G, bool Master, int K>
-__global__ void __launch_bounds__(kThreads, 5) adamw_8bit_kernel(const __grid_constant__ Table<K> table) {
+__global__ void __launch_bounds__(kThreads8, 5) adamw_8bit_kernel(const __grid_constant__ Table<K> table) {
   const Hyper& h = table.h;
   const int number = find_tensor(table);
   const Tensor& t = table.t[number];
@@ -455,10 +465,11 @@ __global__ void __launch_bounds__(kThreads, 5) adamw_8bit_kernel(const __grid_co
   c.left = (int)min((int64_t)kChunk8, t.n - first);
   c.place = (uint32_t)first;
   c.seed = t.seed + (uint32_t)(first >> 32) * 0xBB67AE85u;
+  const int lane = threadIdx.x & 31;
   const int at = (threadIdx.x >> 5) * kBlock;
   if (at >= c.left) return;
-  if (all_wide<P, G, Master>(t, 4) && at + kBlock <= c.left) c.template step<true>(h, c.template fetch<true>(at), at);
-  else c.template step<false>(h, c.template fetch<false>(at), at);
+  if (all_wide<P, G, Master>(t, 4) && at + kBlock <= c.left) c.template step<true>(h, c.template fetch<true>(at + lane * 4), at + lane * 4);
+  else c.template step<false>(h, c.template fetch<false>(at + lane * 4), at + lane * 4);
 }
 
 template <int K> int launch_table(const Table<K>& table, uint32_t blocks, int p_type, int g_type, bool master, int bits, cudaStream_t st) {
@@ -468,7 +479,7 @@ template <int K> int launch_table(const Table<K>& table, uint32_t blocks, int p_
       using G = decltype(g);
       auto go = [&](auto has) {
         constexpr bool M = decltype(has)::value && sizeof(P) == 2;
-        if (bits == 8) adamw_8bit_kernel<P, G, M, K><<<blocks, kThreads, 0, st>>>(table);
+        if (bits == 8) adamw_8bit_kernel<P, G, M, K><<<blocks, kThreads8, 0, st>>>(table);
         else adamw_kernel<P, G, M, K><<<blocks, kThreads, 0, st>>>(table);
       };
       if (master) go(std::true_type());
