@@ -11,7 +11,7 @@
 // (join kernel) between blocks, always in the order of the tokens.  Rows that no token names are filled with zeros by further
 // blocks of the same launch.
 //
-// Three ways to sort, by the number of tokens: up to 1024, every block that sums sorts all of them itself (one launch for
+// Three ways to sort, by the number of tokens: up to 2048, every block that sums sorts all of them itself (one launch for
 // the whole gradient where one block can sum them); up to 65536, a cluster of eight blocks sorts in its shared memory; above, tiles of
 // 2048 tokens are counted, scanned and scattered digit by digit.
 #include <cooperative_groups.h>
@@ -392,14 +392,13 @@ embedding_scatter_kernel(Tokens tokens, const uint32_t* __restrict__ keys, const
 // ---- sums ----------------------------------------------------------------------------------------------------------
 
 constexpr int kSpan = 2048;               // sorted tokens of a block, at most
-constexpr int kLocalItems = 4;
-constexpr int kLocal = kThreads * kLocalItems;  // tokens that every block sorts itself
+constexpr int kLocal = kThreads * 8;      // tokens that every block sorts itself
 constexpr int kFillRows = 1024;           // rows of a block that fills, at most
 
 struct SumArgs {
-  Tokens tokens;           // `local`: sorted in the block
-  int local, passes, bits;
-  const uint32_t* keys;    // else sorted before; entries of key `rows` are left out
+  Tokens tokens;
+  int passes, bits;
+  const uint32_t* keys;    // sorted (unless the blocks sort themselves); entries of key `rows` are left out
   const uint32_t* places;
   const void* grad;
   int64_t grad_stride;
@@ -481,19 +480,19 @@ __device__ __forceinline__ int64_t warp_lower_bound(const uint32_t* keys, int64_
 }
 
 // zeros in those rows from `first` on that no token names
-template <typename TO> __device__ __forceinline__ void fill_rows(const SumArgs& a, int64_t first, uint32_t* named, int64_t* range) {
+template <typename TO, bool Local> __device__ __forceinline__ void fill_rows(const SumArgs& a, int64_t first, uint32_t* named, int64_t* range) {
   const int64_t last = min(first + a.fill_rows, a.tokens.rows);
   for (int i = threadIdx.x; i < kFillRows / 32; i += kThreads) named[i] = 0;
-  if (!a.local && threadIdx.x < 64) {
+  if (!Local && threadIdx.x < 64) {
     const int64_t at = warp_lower_bound(a.keys, a.tokens.n, (uint32_t)(threadIdx.x < 32 ? first : last));
     range[threadIdx.x >> 5] = at;
   }
   __syncthreads();
-  const int64_t lo = a.local ? 0 : range[0], hi = a.local ? a.tokens.n : range[1];
-  if (hi - lo <= 4096) {  // few tokens: all of them, the first of a row marking it
+  const int64_t lo = Local ? 0 : range[0], hi = Local ? a.tokens.n : range[1];
+  if (Local || hi - lo <= 4096) {  // few tokens: all of them, the first of a row marking it
     for (int64_t i = lo + threadIdx.x; i < hi; i += kThreads) {
-      const uint32_t key = a.local ? a.tokens.key(i) : a.keys[i];
-      if (key >= first && key < last && (a.local || i == lo || a.keys[i - 1] != key)) atomicOr(&named[(key - first) >> 5], 1u << ((key - first) & 31));
+      const uint32_t key = Local ? a.tokens.key(i) : a.keys[i];
+      if (key >= first && key < last && (Local || i == lo || a.keys[i - 1] != key)) atomicOr(&named[(key - first) >> 5], 1u << ((key - first) & 31));
     }
   } else {  // many: a search for every row
     for (int r = threadIdx.x; r < last - first; r += kThreads) {
@@ -546,13 +545,16 @@ template <int N> struct SumShared {
   int64_t range[2];
 };
 
-template <typename TI, typename TO, int N, bool Whole, bool Add> __global__ void __launch_bounds__(kThreads) embedding_sum_kernel(SumArgs a) {
+// Local: every block sorts all tokens itself.  (The sort's registers would cost the other form its fourth block on an SM: 1.5M samples 104
+// against 93 us.)
+template <typename TI, typename TO, int N, bool Whole, bool Add, bool Local>
+__global__ void __launch_bounds__(kThreads) embedding_sum_kernel(SumArgs a) {
   __shared__ SumShared<N> s;
   constexpr int kBatch = Add || !Whole ? 4 : 8;  // rows in flight
   griddep_wait();
   const int64_t sum_blocks = a.n_blocks * a.n_cols;
   if (blockIdx.x >= sum_blocks) {
-    fill_rows<TO>(a, ((int64_t)blockIdx.x - sum_blocks) * a.fill_rows, s.named, s.range);
+    fill_rows<TO, Local>(a, ((int64_t)blockIdx.x - sum_blocks) * a.fill_rows, s.named, s.range);
     return;
   }
   const int64_t block = blockIdx.x / a.n_cols, block0 = block * a.workers * a.share;
@@ -560,9 +562,10 @@ template <typename TI, typename TO, int N, bool Whole, bool Add> __global__ void
   const uint32_t none = (uint32_t)a.tokens.rows;
   if (threadIdx.x == 0) s.valid = 0;
   int off = 0;  // of the block's first token in s.token, and in s.key of the token before it
-  if (a.local) {
+  if constexpr (Local) {
     off = (int)block0;
-    sort_block<kThreads / 32, kLocalItems>(s.sort, a.tokens, a.passes, a.bits, s.key + 1, s.token);
+    if (a.tokens.n <= kLocal / 2) sort_block<kThreads / 32, 4>(s.sort, a.tokens, a.passes, a.bits, s.key + 1, s.token);
+    else sort_block<kThreads / 32, 8>(s.sort, a.tokens, a.passes, a.bits, s.key + 1, s.token);
     if (threadIdx.x == 0) s.key[0] = s.key[a.tokens.n + 1] = kNoKey;
   } else {
     for (int i = threadIdx.x; i < count; i += kThreads) {
@@ -884,7 +887,6 @@ extern "C" int gnr_embedding_grad(const void* grad, int grad_type, int dim, int6
   }
   SumArgs a{};
   a.tokens = tokens;
-  a.local = local;
   a.passes = p.passes;
   a.bits = p.bits;
   a.keys = u32(p.keys[cur]);
@@ -910,8 +912,12 @@ extern "C" int gnr_embedding_grad(const void* grad, int grad_type, int dim, int6
       using TI = decltype(ti);
       using TO = decltype(to);
       constexpr int N = 16 / sizeof(TI);
-      auto* sum = vec ? accumulate ? embedding_sum_kernel<TI, TO, N, true, true> : embedding_sum_kernel<TI, TO, N, true, false>
-                      : accumulate ? embedding_sum_kernel<TI, TO, 4, false, true> : embedding_sum_kernel<TI, TO, 4, false, false>;
+      auto pick = [&](auto is_local) {
+        constexpr bool L = decltype(is_local)::value;
+        return vec ? accumulate ? embedding_sum_kernel<TI, TO, N, true, true, L> : embedding_sum_kernel<TI, TO, N, true, false, L>
+                   : accumulate ? embedding_sum_kernel<TI, TO, 4, false, true, L> : embedding_sum_kernel<TI, TO, 4, false, false, L>;
+      };
+      auto* sum = local ? pick(std::true_type()) : pick(std::false_type());
       auto* join = vec ? accumulate ? embedding_join_kernel<TO, N, true, true> : embedding_join_kernel<TO, N, true, false>
                        : accumulate ? embedding_join_kernel<TO, 4, false, true> : embedding_join_kernel<TO, 4, false, false>;
       GNR_CUDA_OK((cudaError_t)gnr_launch(sum, (unsigned)blocks, kThreads, 0, st, !local, a));

@@ -131,7 +131,7 @@ def test_gradient(dtype, t, v, d, spread):
 
 
 # where the way of sorting, the number of blocks or the number of passes changes, and one beside it
-BORDERS = [(n + k, v, d) for n, v, d in ((672, 11500, 48), (1024, 11500, 48), (8192, 511, 4), (16384, 512, 4), (32768, 262143, 4), (65536, 262144, 4),
+BORDERS = [(n + k, v, d) for n, v, d in ((672, 11500, 48), (1024, 11500, 48), (2048, 11500, 48), (8192, 511, 4), (16384, 512, 4), (32768, 262143, 4), (65536, 262144, 4),
                                          (2048 * 40, 3, 1)) for k in (0, 1)]
 
 

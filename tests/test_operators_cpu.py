@@ -40,12 +40,12 @@ def test_c_entries_refuse():
     assert lib.gnr_embedding_lookup(p, 0, 5, 4, 3, p, 64, 3, 1.0, p, 4, None) < 0  # rows that overlap
     assert lib.gnr_embedding_lookup(None, 0, 5, 4, 4, p, 64, 3, 1.0, p, 4, None) < 0
     assert lib.gnr_embedding_lookup(None, 0, 5, 4, 4, None, 64, 0, 1.0, None, 4, None) == 0  # nothing to do
-    assert lib.gnr_embedding_grad(p, 0, 4, 4, p, 64, 2000, 5, -1, 1.0, 0, p, 0, 4, p, 16, None) < 0 and b"workspace" in lib.gnr_last_error()
+    assert lib.gnr_embedding_grad(p, 0, 4, 4, p, 64, 5000, 5, -1, 1.0, 0, p, 0, 4, p, 16, None) < 0 and b"workspace" in lib.gnr_last_error()
     assert lib.gnr_embedding_grad(p, 0, 4, 4, p, 64, 3, 5, -1, 1.0, 0, p, 0, 3, p, 1 << 30, None) < 0
     assert lib.gnr_embedding_grad(p, 0, 4, 4, p, 64, 3, 5, -1, 1.0, 0, p, 7, 4, p, 1 << 30, None) < 0
     assert lib.gnr_embedding_grad(p, 0, 4, 4, None, 64, 3, 5, -1, 1.0, 0, p, 0, 4, p, 1 << 30, None) < 0
-    assert lib.gnr_embedding_grad(p, 0, 4, 4, p, 64, 2000, 5, -1, 1.0, 0, p, 0, 4, None, 1 << 30, None) < 0
-    assert lib.gnr_embedding_grad(p, 0, 4, 4, p, 64, 2000, 5, -1, 1.0, 0, p, 0, 4, C.c_void_p(264), 1 << 30, None) < 0  # not on 16 bytes
+    assert lib.gnr_embedding_grad(p, 0, 4, 4, p, 64, 5000, 5, -1, 1.0, 0, p, 0, 4, None, 1 << 30, None) < 0
+    assert lib.gnr_embedding_grad(p, 0, 4, 4, p, 64, 5000, 5, -1, 1.0, 0, p, 0, 4, C.c_void_p(264), 1 << 30, None) < 0  # not on 16 bytes
 
 
 def test_adamw_entry_refuses():
