@@ -464,7 +464,8 @@ typedef struct GnrAdamwTensor {
 /* One AdamW step (decoupled weight decay) over all of them, for tensors of one parameter type and one gradient type:
  *   m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2,
  *   p = p (1 - lr weight_decay) - lr / (1 - beta1^step) m / (sqrt(v / (1 - beta2^step)) + eps),
- * in fp32.  ``state_bits`` 32 or 8; ``step`` counts from 1.  ``tensors_h`` is read before the call returns. */
+ * in fp32.  ``state_bits`` 32 or 8; ``step`` counts from 1.  ``tensors_h`` is read before the call returns; a launch that is
+ * captured into a CUDA graph repeats this call's addresses, count and rates. */
 int gnr_adamw_step(const GnrAdamwTensor* tensors_h, int n_tensors, int param_type, int grad_type, int state_bits, int64_t step,
                    double lr, double beta1, double beta2, double eps, double weight_decay, uint32_t seed, void* stream);
 

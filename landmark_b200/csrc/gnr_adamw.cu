@@ -537,7 +537,7 @@ extern "C" int gnr_adamw_step(const GnrAdamwTensor* tensors_h, int n_tensors, in
   }
   for (int k = 0; k < n_tensors; ++k) {
     const GnrAdamwTensor& t = tensors_h[k];
-    if (t.n < 0 || t.n > ((int64_t)0x7fffffff * kChunk) ||
+    if (t.n < 0 || t.n > (int64_t)0x7fffffff * (state_bits == 8 ? kChunk8 : kChunk) ||
         (t.n > 0 && (!t.param || !t.grad || !t.exp_avg || !t.exp_avg_sq || (state_bits == 8 && (!t.exp_avg_scale || !t.exp_avg_sq_scale)))) ||
         (t.master != nullptr) != master) {
       gnr_set_error("gnr_adamw_step: tensor %d of %lld values: null pointer, or some tensors have a 32-bit copy and others none", k, (long long)t.n);

@@ -47,12 +47,12 @@ def batch(spec, model, seed=0):
     return rays, torch.rand((rays.shape[0], 3), generator=gen, device="cuda"), codes
 
 
-@pytest.mark.parametrize("white_bg", [True, False])
-def test_gradients_match_the_formula(white_bg):
+@pytest.mark.parametrize("white_bg,mode", [(True, {}), (False, {}), (True, {"mlp_mode": 2, "app_plane_fp16": True, "density_lattice": True})])
+def test_gradients_match_the_formula(white_bg, mode):
     from landmark_b200.appearance import AppearanceFit
 
     spec = scene()
-    model = cuda_model(spec)
+    model = cuda_model(spec, **mode)
     rays, colors, codes = batch(spec, model)
     fit = AppearanceFit(model, network=True)
     params = fit._parameters()
