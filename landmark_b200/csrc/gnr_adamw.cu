@@ -43,12 +43,18 @@ struct Tensor {
   uint32_t seed;
 };
 
+// A number twice, as the packed operations take it: from the kernel's arguments without a move.
+struct alignas(8) Twice {
+  float x, y;
+};
+
 struct Hyper {
-  float b1, b1c, b2, b2c;  // betas and 1 - betas
-  float keep;              // 1 - lr * weight decay
-  float rate;              // lr / (1 - b1^t)
-  float c2_inv;            // 1 / sqrt(1 - b2^t)
-  float eps;
+  Twice b1, b1c, b2, b2c;  // betas and 1 - betas
+  Twice keep;              // 1 - lr * weight decay
+  Twice rate;              // -lr / (1 - b1^t)
+  Twice c2_inv;            // 1 / sqrt(1 - b2^t)
+  Twice eps;
+  Twice minus_one, two, eighth;
 };
 
 template <int K> struct Table {
@@ -80,6 +86,11 @@ __device__ __forceinline__ Two two(float x, float y) {
   return r;
 }
 __device__ __forceinline__ Two two(float x) { return two(x, x); }
+__device__ __forceinline__ Two two(const Twice& x) {
+  Two r;
+  r.v = *reinterpret_cast<const unsigned long long*>(&x);
+  return r;
+}
 __device__ __forceinline__ void split(Two a, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(a.v)); }
 __device__ __forceinline__ Two mul2(Two a, Two b) {
   Two r;
@@ -106,12 +117,12 @@ __device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
   return r;
 }
-__device__ __forceinline__ Two sub2(Two a, Two b) { return fma2(b, two(-1.0f), a); }
+__device__ __forceinline__ Two sub2(const Hyper& h, Two a, Two b) { return fma2(b, two(h.minus_one), a); }
 
 // m and v after the gradient g
 __device__ __forceinline__ void moments(const Hyper& h, float g, float& m, float& v) {
-  m = __fadd_rn(__fmul_rn(h.b1, m), __fmul_rn(h.b1c, g));
-  v = __fadd_rn(__fmul_rn(h.b2, v), __fmul_rn(__fmul_rn(h.b2c, g), g));
+  m = __fadd_rn(__fmul_rn(h.b1.x, m), __fmul_rn(h.b1c.x, g));
+  v = __fadd_rn(__fmul_rn(h.b2.x, v), __fmul_rn(__fmul_rn(h.b2c.x, g), g));
 }
 
 // 1 / x of a normal number, within one unit of the last place
@@ -122,7 +133,7 @@ __device__ __forceinline__ float quick_rcp(float x) {
 }
 
 __device__ __forceinline__ float stepped(const Hyper& h, float x, float m, float root) {
-  return x * h.keep - h.rate * (m * quick_rcp(root * h.c2_inv + h.eps));
+  return fmaf(h.rate.x, m * quick_rcp(fmaf(root, h.c2_inv.x, h.eps.x)), x * h.keep.x);
 }
 
 // Four values of a thread: the neighbours from i on, or (not Wide) those kThreads apart from i on that lie before `end`, 0 for the others.
@@ -264,6 +275,12 @@ __device__ __forceinline__ void store_codes(uint8_t* at, bool whole, int count, 
 // value from 2^-6 on.  Below, the codes are 2^-9 apart as in the binade above: 2^-6 is added (kShift) and 8 taken off.
 constexpr float kShift = 0.015625f;
 
+// the signs of four numbers as those of four codes
+__device__ __forceinline__ uint32_t signs(const float (&m)[4]) {
+  const uint32_t low = __byte_perm(__float_as_uint(m[0]), __float_as_uint(m[1]), 0x73), high = __byte_perm(__float_as_uint(m[2]), __float_as_uint(m[3]), 0x73);
+  return __byte_perm(low, high, 0x5410) & 0x80808080u;
+}
+
 // |m| * inv rounded up where a uniform u = (r + 1/2) / 2^16 is below the part of it past the code below: adding 1 - u of a code, less
 // one, to the bits carries into the code in just these cases (u has 17 bits, the part 20; rounded upwards where the shift cuts it).
 __device__ __forceinline__ void codes_of_m(const float (&m)[2], Two inv, const uint32_t (&r32)[2], uint32_t (&code)[2]) {
@@ -278,12 +295,12 @@ __device__ __forceinline__ void codes_of_m(const float (&m)[2], Two inv, const u
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
     const uint32_t at = (__float_as_uint(z[k]) + ((~r32[k] & 0xffffu) << 4 | 7u)) >> 20;
-    code[k] = (at - (y[k] < kShift ? 968u : 960u)) | (__float_as_uint(m[k]) >> 24 & 0x80u);
+    code[k] = at - (y[k] < kShift ? 968u : 960u);
   }
 }
 
 // root * inv rounded so that the mean of its square is kept: up where u < (y^2 - low^2) / ((low + step)^2 - low^2)
-__device__ __forceinline__ void codes_of_root(const float (&root)[2], Two inv, const uint32_t (&r32)[2], uint32_t (&code)[2]) {
+__device__ __forceinline__ void codes_of_root(const Hyper& h, const float (&root)[2], Two inv, const uint32_t (&r32)[2], uint32_t (&code)[2]) {
   float y[2], shift[2], z[2], a[2], b[2];
   split(mul2(two(root[0], root[1]), inv), y[0], y[1]);
 #pragma unroll
@@ -294,11 +311,11 @@ __device__ __forceinline__ void codes_of_root(const float (&root)[2], Two inv, c
   const Two yy = two(y[0], y[1]), shifts = two(shift[0], shift[1]);
   split(add2_zero(yy, shifts), z[0], z[1]);
   const uint32_t z0 = __float_as_uint(z[0]), z1 = __float_as_uint(z[1]);
-  const Two low = sub2(two(__uint_as_float(z0 & ~0xfffffu), __uint_as_float(z1 & ~0xfffffu)), shifts);
-  const Two step = mul2(two(__uint_as_float(z0 & 0x7f800000u), __uint_as_float(z1 & 0x7f800000u)), two(0.125f));
-  const Two u = add2(two(__uint_as_float(0x3f800040u | (r32[0] >> 16) << 7), __uint_as_float(0x3f800040u | (r32[1] >> 16) << 7)), two(-1.0f));
-  split(mul2(mul2(u, fma2(two(2.0f), low, step)), step), a[0], a[1]);
-  split(mul2(sub2(yy, low), add2(yy, low)), b[0], b[1]);
+  const Two low = sub2(h, two(__uint_as_float(z0 & ~0xfffffu), __uint_as_float(z1 & ~0xfffffu)), shifts);
+  const Two step = mul2(two(__uint_as_float(z0 & 0x7f800000u), __uint_as_float(z1 & 0x7f800000u)), two(h.eighth));
+  const Two u = add2(two(__uint_as_float(0x3f800040u | (r32[0] >> 16) << 7), __uint_as_float(0x3f800040u | (r32[1] >> 16) << 7)), two(h.minus_one));
+  split(mul2(mul2(u, fma2(two(h.two), low, step)), step), a[0], a[1]);
+  split(mul2(sub2(h, yy, low), add2(yy, low)), b[0], b[1]);
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
     const uint32_t at = (__float_as_uint(z[k]) >> 20) - (y[k] < kShift ? 968u : 960u) + (a[k] < b[k] ? 1u : 0u);
@@ -382,7 +399,7 @@ template <typename P, typename G, bool Master> struct Chunk8 {
         float d0, d1;
         split(fma2(two(root[s][k], root[s][k + 1]), two(h.c2_inv), two(h.eps)), d0, d1);
         const Two q = mul2(two(m[s][k], m[s][k + 1]), two(quick_rcp(d0), quick_rcp(d1)));
-        split(fma2(two(-h.rate), q, mul2(two(x[s][k], x[s][k + 1]), two(h.keep))), x[s][k], x[s][k + 1]);
+        split(fma2(two(h.rate), q, mul2(two(x[s][k], x[s][k + 1]), two(h.keep))), x[s][k], x[s][k + 1]);
         m_bits = max(max(m_bits, __float_as_uint(m[s][k]) & 0x7fffffffu), __float_as_uint(m[s][k + 1]) & 0x7fffffffu);
         v_bits = max(max(v_bits, __float_as_uint(root[s][k])), __float_as_uint(root[s][k + 1]));
       }
@@ -422,10 +439,11 @@ template <typename P, typename G, bool Master> struct Chunk8 {
         const float mk[2] = {m[s][k], m[s][k + 1]}, rk[2] = {root[s][k], root[s][k + 1]};
         uint32_t m_code[2], v_code[2];
         codes_of_m(mk, two(m_inv), r32, m_code);
-        codes_of_root(rk, two(v_inv), r32, v_code);
+        codes_of_root(h, rk, two(v_inv), r32, v_code);
         m_codes |= (m_code[0] | m_code[1] << 8) << (8 * k);
         v_codes |= (v_code[0] | v_code[1] << 8) << (8 * k);
       }
+      m_codes |= signs(m[s]);
       if (odd) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
@@ -545,14 +563,18 @@ extern "C" int gnr_adamw_step(const GnrAdamwTensor* tensors_h, int n_tensors, in
     }
   }
   Hyper h;
-  h.b1 = (float)beta1;
-  h.b1c = (float)(1.0 - beta1);
-  h.b2 = (float)beta2;
-  h.b2c = (float)(1.0 - beta2);
-  h.keep = (float)(1.0 - lr * weight_decay);
-  h.rate = (float)(lr / (1.0 - pow(beta1, (double)step)));
-  h.c2_inv = (float)(1.0 / sqrt(1.0 - pow(beta2, (double)step)));
-  h.eps = (float)eps;
+  auto twice = [](double x) { return Twice{(float)x, (float)x}; };
+  h.b1 = twice(beta1);
+  h.b1c = twice(1.0 - beta1);
+  h.b2 = twice(beta2);
+  h.b2c = twice(1.0 - beta2);
+  h.keep = twice(1.0 - lr * weight_decay);
+  h.rate = twice(-lr / (1.0 - pow(beta1, (double)step)));
+  h.c2_inv = twice(1.0 / sqrt(1.0 - pow(beta2, (double)step)));
+  h.eps = twice(eps);
+  h.minus_one = twice(-1.0);
+  h.two = twice(2.0);
+  h.eighth = twice(0.125);
   const uint32_t of_step = hash32((uint32_t)step, seed + (uint32_t)((uint64_t)step >> 32) * 0xBB67AE85u);
   const cudaStream_t st = (cudaStream_t)stream;
   return n_tensors <= kSmall ? step_all<kSmall>(tensors_h, n_tensors, h, param_type, grad_type, master, state_bits, of_step, st)

@@ -545,7 +545,7 @@ template <int N> struct SumShared {
 template <typename TI, typename TO, int N, bool Whole, bool Add, bool Local>
 __global__ void __launch_bounds__(kThreads) embedding_sum_kernel(SumArgs a) {
   __shared__ SumShared<N> s;
-  constexpr int kBatch = Add || !Whole ? 4 : 8;  // rows in flight
+  constexpr int kBatch = Add ? (Whole ? 2 : 4) : 8;  // rows in flight
   griddep_wait();
   const int64_t sum_blocks = a.n_blocks * a.n_cols;
   if (blockIdx.x >= sum_blocks) {
