@@ -147,6 +147,20 @@ def test_gradient_at_borders(t, v, d, spread):
     assert torch.equal(got, embedding_backward(g, idx, v))
 
 
+def test_many_tokens():
+    """Twenty million tokens: whole numbers, so that every sum is exact whatever its order."""
+    from landmark_b200.embedding import embedding_backward
+
+    t, v = 20_000_003, 11500
+    g = torch.ones((t, 4), device="cuda")
+    for idx in (torch.arange(t, device="cuda") % v, torch.arange(t, device="cuda") // 1_000_000, torch.zeros(t, dtype=torch.int64, device="cuda")):
+        got = embedding_backward(g, idx, v)
+        assert torch.equal(got, torch.bincount(idx, minlength=v).float()[:, None].expand(v, 4)) or float(got.max()) >= 2 ** 24
+        if float(got.max()) >= 2 ** 24:  # one row: past the whole numbers that fp32 counts singly
+            n = torch.bincount(idx, minlength=v).double()[:, None]
+            assert bool(((got.double() - n).abs() <= n * 1000 * U).all())
+
+
 @pytest.mark.parametrize("d", [1, 2, 3, 5, 255, 257, 1023, 1025, 4100])
 def test_gradient_of_odd_widths(d):
     from landmark_b200.embedding import embedding_backward
