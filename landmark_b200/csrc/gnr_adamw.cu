@@ -176,6 +176,8 @@ template <typename P, typename G, bool Master> __device__ __forceinline__ bool a
          (uintptr_t)t.v % state_align == 0 && (!Master || (uintptr_t)t.master % 16 == 0);
 }
 
+// Bound by HBM: 16 values of every array in flight a thread; 335M fp32 values with gradients take 1355 us, 6.9 TB/s (with divisions for the two
+// quotients 1517 us), 60M bf16 values with fp32 copies in 300 tensors 250 us, 6.7 TB/s.
 template <typename P, typename G, bool Master, int K>
 __global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__ Table<K> table) {
   const Hyper& h = table.h;
@@ -331,7 +333,6 @@ template <typename X, typename G> struct Part {
   float m_scale, v_scale;
 };
 
-// A thread block's values of a tensor with 8-bit states; all places count from their beginning.
 // 448 / top, 0 for 0: the quick reciprocal and one Newton step (rounded like the exact one but for some in a million)
 __device__ __forceinline__ float scale_up(float top) {
   if (top > 1e30f) return __fmul_rn(__frcp_rn(top), kTop);
@@ -339,6 +340,7 @@ __device__ __forceinline__ float scale_up(float top) {
   return top > 0.0f ? __fmul_rn(__fmaf_rn(r, __fmaf_rn(-top, r, 1.0f), r), kTop) : 0.0f;
 }
 
+// A thread block's values of a tensor with 8-bit states; all places count from their beginning.
 template <typename P, typename G, bool Master> struct Chunk8 {
   using X = std::conditional_t<Master, float, P>;
   P* p_at;
@@ -461,11 +463,11 @@ template <typename P, typename G, bool Master> struct Chunk8 {
   }
 };
 
-// A warp takes one block of 256 values.  Bound by its instructions, 89 a value with the packed fp32 ones counted for two (85 % of the issue
-// slots), and by the power they draw: 335M fp32 values take 991 us at 1965 MHz, 5.4 TB/s, and 1080 to 1150 us in a long run, where the power
+// A warp takes one block of 256 values.  Bound by its instructions, 89 a value with the packed fp32 ones counted for two (87 % of the issue
+// slots), and by the power they draw: 335M fp32 values take 966 us at 1965 MHz, 5.6 TB/s, and 1040 to 1140 us in a long run, where the power
 // cap holds the clock at 1.65 to 1.75 GHz.  Five thread blocks to an SM hide the loads better than a longer run of blocks with the
 // next one's loads ahead of the work (1058 against 948 us on zeros), six spill (1000).  A root by Newton's step from the quick reciprocal
-// root, with a way out for its range, saves instructions and loses their overlap (1091 against 997 us).
+// root, with a way out for its range, takes as long (954 us), in a pass of its own longer (1091).
 template <typename P, typename G, bool Master, int K>
 __global__ void __launch_bounds__(kThreads8, 5) adamw_8bit_kernel(const __grid_constant__ Table<K> table) {
   const Hyper& h = table.h;

@@ -114,7 +114,8 @@ template <int Items> __device__ __forceinline__ int tile_place(int j) {
   return (threadIdx.x >> 5) * (32 * Items) + j * 32 + (threadIdx.x & 31);
 }
 
-// lanes whose digit is this lane's
+// lanes whose digit is this lane's.  (One vote per bit instead: 1.5M uniform digits sorted in 100 - 44 us instead of 119 - 44, but runs of one code in
+// 79 - 44 instead of 60 - 44, and those are what samples of rays bring.)
 __device__ __forceinline__ uint32_t digit_peers(uint32_t digit, bool there) { return __match_any_sync(0xffffffffu, there ? digit : kNoKey); }
 
 // Ranks of a tile's tokens among the tokens of the same digit, in the tile's order (the first `n` places hold one).  Afterwards
@@ -540,6 +541,8 @@ template <int N> struct SumShared {
   int64_t range[2];
 };
 
+// Bound by the latency of rows fetched from anywhere, eight of them in flight a thread: 1.5M rows of 48 fp32 55 us, 5.2 TB/s (four in flight 63, 16 65 us); with
+// Add two, beside the rows that they are added to (16384 tokens of 2048 bf16 into fp32 rows 53 us, 5.7 TB/s).
 // Local: every block sorts all tokens itself.  (The sort's registers would cost the other form its fourth block on an SM: 1.5M samples 104
 // against 93 us.)
 template <typename TI, typename TO, int N, bool Whole, bool Add, bool Local>
