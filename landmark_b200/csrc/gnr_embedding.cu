@@ -114,8 +114,8 @@ template <int Items> __device__ __forceinline__ int tile_place(int j) {
   return (threadIdx.x >> 5) * (32 * Items) + j * 32 + (threadIdx.x & 31);
 }
 
-// lanes whose digit is this lane's.  (One vote per bit instead: 1.5M uniform digits sorted in 100 - 44 us instead of 119 - 44, but runs of one code in
-// 79 - 44 instead of 60 - 44, and those are what samples of rays bring.)
+// lanes whose digit is this lane's.  The more digits a warp holds, the longer it takes: the gradient of 1.5M tokens of 4 values takes 60 us
+// for runs of one code (what samples of rays bring) and 119 us for uniform ones; with one vote per bit instead 79 and 100.
 __device__ __forceinline__ uint32_t digit_peers(uint32_t digit, bool there) { return __match_any_sync(0xffffffffu, there ? digit : kNoKey); }
 
 // Ranks of a tile's tokens among the tokens of the same digit, in the tile's order (the first `n` places hold one).  Afterwards
