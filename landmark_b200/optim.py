@@ -82,6 +82,8 @@ class AdamWTensors:
             if len(tensors) != len(sizes):
                 raise ValueError(f"{len(tensors)} {name} for {len(sizes)} params")
             for k, (t, n) in enumerate(zip(tensors, want)):
+                if not isinstance(t, torch.Tensor):
+                    raise TypeError(f"{name}[{k}] must be a tensor, got {type(t).__name__}")
                 if t.dtype != dtype or t.device != self.device or t.numel() != n or t.layout is not torch.strided or not t.is_contiguous():
                     raise ValueError(f"{name}[{k}] must be {n} contiguous values of {dtype} on {self.device}, got {tuple(t.shape)} of {t.dtype} "
                                      f"on {t.device}")
@@ -164,7 +166,7 @@ class AdamW(torch.optim.Optimizer):
         if not lr >= 0 or not eps >= 1e-30 or not weight_decay >= 0 or not all(0 <= b < 1 for b in betas):
             raise ValueError(f"lr {lr}, betas {betas}, eps {eps} (at least 1e-30), weight_decay {weight_decay}")
         self.state_bits, self.master_weights, self.seed = state_bits, master_weights, seed
-        self._sets: dict = {}  # (group, device, type) -> (parameters, their states by name, AdamWTensors)
+        self._sets: dict = {}  # (group, device, type) -> (parameters, their states, these by name, AdamWTensors)
         super().__init__(params, {"lr": lr, "betas": betas, "eps": eps, "weight_decay": weight_decay})
 
     def add_param_group(self, param_group):
@@ -205,17 +207,19 @@ class AdamW(torch.optim.Optimizer):
         return s
 
     def _tensors(self, key, params) -> Tuple[list, AdamWTensors]:
-        """States of ``params`` and the checked set of them, made again where a state has been replaced."""
-        states = [self._state_of(p) for p in params]
-        names = [n for n in ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale", "master") if n in states[0]]
-        parts = {n: [s[n] for s in states] for n in names}
+        """States of ``params`` and the checked set of them, made again where a parameter or state has been replaced."""
         old = self._sets.get(key)
-        if old is not None and old[2].starts == list(map(_address, params)) and old[1].keys() == parts.keys() and all(
-                len(old[1][n]) == len(parts[n]) and all(map(operator.is_, old[1][n], parts[n])) for n in names):
-            return states, old[2]
+        if old is not None:
+            old_params, states, parts, made = old
+            if (len(old_params) == len(params) and all(map(operator.is_, old_params, params)) and made.starts == list(map(_address, params))
+                    and all(map(operator.is_, map(self.state.get, params), states))
+                    and all(all(map(operator.is_, [s.get(name) for s in states], kept)) for name, kept in parts.items())):
+                return states, made
+        states = [self._state_of(p) for p in params]
+        parts = {n: [s.get(n) for s in states] for n in ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale", "master") if n in states[0]}
         made = AdamWTensors([p.detach() for p in params], parts["exp_avg"], parts["exp_avg_sq"], parts.get("exp_avg_scale"), parts.get("exp_avg_sq_scale"),
                             parts.get("master"))
-        self._sets[key] = (list(params), parts, made)
+        self._sets[key] = (params, states, parts, made)
         return states, made
 
     @torch.no_grad()
@@ -231,8 +235,9 @@ class AdamW(torch.optim.Optimizer):
                     sets.setdefault((number, p.device, p.dtype), []).append(p)
             for k, (key, params) in enumerate(sets.items()):
                 states, tensors = self._tensors(key, params)
-                for t in sorted({s["step"] for s in states}):  # one, unless a parameter had no gradient in some steps
-                    grads = [p.grad if s["step"] == t else None for p, s in zip(params, states)]
+                counts = {s["step"] for s in states}
+                for t in sorted(counts):  # one, unless a parameter had no gradient in some steps
+                    grads = [p.grad if len(counts) == 1 or s["step"] == t else None for p, s in zip(params, states)]
                     tensors.step(grads, step=int(t) + 1, lr=float(group["lr"]), betas=group["betas"], eps=group["eps"],
                                  weight_decay=group["weight_decay"], seed=self.seed + 0x3C6EF372 * (2 * number + 1) + k)
                 for s in states:
