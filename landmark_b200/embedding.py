@@ -161,7 +161,7 @@ class _EmbeddingBackward(torch.autograd.Function):
 
 
 def _new_gradient(grad, indices, num_rows, scale, padding_idx, dtype):
-    return _gradient(grad, indices, scale, padding_idx, torch.empty((num_rows, grad.shape[-1]), dtype=dtype, device=grad.device), False)
+    return _gradient(grad, indices, scale, padding_idx, grad.new_empty((num_rows, grad.shape[-1]), dtype=dtype), False)
 
 
 def _check_padding(padding_idx: int, rows: int) -> int:
@@ -199,8 +199,9 @@ def embedding_backward(grad_output: torch.Tensor, indices: torch.Tensor, num_row
     if out is None:
         if accumulate:
             raise ValueError("accumulate needs out")
-        dtype = grad_output.dtype if dtype is None else dtype
-        if dtype not in _TYPES:
+        if dtype is None:
+            dtype = grad_output.dtype
+        elif dtype not in _TYPES:
             raise TypeError(f"dtype must be float32, float16 or bfloat16, got {dtype}")
         if grad_output.requires_grad and torch.is_grad_enabled():
             return _EmbeddingBackward.apply(grad_output, indices, num_rows, float(scale), padding_idx, dtype)

@@ -94,6 +94,7 @@ class AdamWTensors:
         self._table[:, _N] = sizes
         self._table[:, _N + 1] = np.arange(len(sizes))
         self.starts = self._table[:, 0].tolist()  # addresses of the parameters
+        self._words = C.c_int64 * self._table.size
         # the memory that the table names stays, whatever becomes of the tensors
         self._kept = [t.detach() for tensors, _, _ in self._tensors.values() for t in tensors]
 
@@ -106,13 +107,16 @@ class AdamWTensors:
         if list(map(_address, self.params)) != self.starts:
             raise ValueError("a parameter has been given other memory since it was checked")
         index = self.device.index
-        table = self._table.copy()
+        table = self._words.from_buffer_copy(self._table)  # a copy for this call
         try:  # all there and as they should be
             kinds = {g.dtype for g in grads}
             plain = (list(map(_numel, grads)) == self.sizes and set(map(_get_device, grads)) == {index} and len(kinds) == 1
                      and all(map(_is_contiguous, grads)) and kinds <= _TYPES.keys())
-            if plain:
-                table[:, _GRAD] = list(map(_address, grads))
+            if plain and len(grads) > 32:
+                np.frombuffer(table, dtype=np.int64)[_GRAD::_WORDS] = list(map(_address, grads))
+            elif plain:
+                for at, address in zip(range(_GRAD, len(table), _WORDS), map(_address, grads)):
+                    table[at] = address
         except (AttributeError, TypeError, RuntimeError):
             plain = False
         if plain:
@@ -124,7 +128,7 @@ class AdamWTensors:
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("an AdamW step cannot be captured into a CUDA graph: a replay would repeat this step's count and rates")
         with _on(index):
-            check(lib.gnr_adamw_step(table.ctypes.data, len(table), _TYPES[self.dtype], _TYPES[kind], self.state_bits, step, lr, betas[0], betas[1],
+            check(lib.gnr_adamw_step(table, len(self.sizes), _TYPES[self.dtype], _TYPES[kind], self.state_bits, step, lr, betas[0], betas[1],
                                      eps, weight_decay, seed & 0xFFFFFFFF, _raw_stream(index)), "gnr_adamw_step")
 
     def _grads(self, grads, table):
@@ -132,7 +136,7 @@ class AdamWTensors:
         kept, kind = [], None
         for k, (g, n) in enumerate(zip(grads, self.sizes)):
             if g is None:
-                table[k, _N] = 0
+                table[k * _WORDS + _N] = 0
                 continue
             if g.get_device() != self.device.index or g.layout is not torch.strided or g.numel() != n:
                 raise ValueError(f"gradient {k} must be {n} dense values on {self.device}, got {tuple(g.shape)} on {g.device}")
@@ -142,7 +146,7 @@ class AdamWTensors:
                 raise TypeError(f"gradients must be of one type, float32, float16 or bfloat16: got {g.dtype} at {k}, {kind} before")
             g = g.contiguous()
             kept.append(g)
-            table[k, _GRAD] = g.data_ptr()
+            table[k * _WORDS + _GRAD] = g.data_ptr()
         return kept, kind
 
 
