@@ -114,8 +114,8 @@ template <int Items> __device__ __forceinline__ int tile_place(int j) {
   return (threadIdx.x >> 5) * (32 * Items) + j * 32 + (threadIdx.x & 31);
 }
 
-// lanes whose digit is this lane's.  The more digits a warp holds, the longer it takes: the gradient of 1.5M tokens of 4 values takes 60 us
-// for runs of one code (what samples of rays bring) and 119 us for uniform ones; with one vote per bit instead 79 and 100.
+// lanes whose digit is this lane's.  The more digits a warp holds, the longer it takes; for runs of one code, what samples of rays bring, the
+// gradient of 1.5M tokens of 4 values takes 60 us, with one vote per bit instead 79.
 __device__ __forceinline__ uint32_t digit_peers(uint32_t digit, bool there) { return __match_any_sync(0xffffffffu, there ? digit : kNoKey); }
 
 // Ranks of a tile's tokens among the tokens of the same digit, in the tile's order (the first `n` places hold one).  Afterwards
@@ -323,10 +323,12 @@ embedding_count_kernel(Tokens tokens, const uint32_t* __restrict__ keys, int shi
   __syncthreads();
 #pragma unroll
   for (int j = 0; j < kItems; ++j) {
-    const bool there = tile0 + tile_place<kItems>(j) < tokens.n;
-    const uint32_t digit = key[j] >> shift & (radix - 1);
-    const uint32_t peers = digit_peers(digit, there);
-    if (there && (peers & ((1u << (threadIdx.x & 31)) - 1u)) == 0) atomicAdd(&s_count[digit], __popc(peers));
+    // one addition for every run of equal digits in the warp
+    const uint32_t digit = tile0 + tile_place<kItems>(j) < tokens.n ? key[j] >> shift & (radix - 1) : kNoKey;
+    const int lane = threadIdx.x & 31;
+    const bool head = __shfl_up_sync(0xffffffffu, digit, 1) != digit || lane == 0;
+    const uint32_t behind = __ballot_sync(0xffffffffu, head) >> lane >> 1;  // heads of later runs
+    if (head && digit != kNoKey) atomicAdd(&s_count[digit], behind ? (uint32_t)__ffs(behind) : 32u - lane);
   }
   __syncthreads();
   for (uint32_t d = threadIdx.x; d < radix; d += kTileWarps * 32) counts[(int64_t)d * n_tiles + blockIdx.x] = s_count[d];
