@@ -347,6 +347,39 @@ def test_copied_and_saved_optimisers_go_on(state_bits):
         opt.load_state_dict(kept[1])
 
 
+def test_closures_schedulers_and_loss_scaling():
+    """What torch builds on an optimiser: a closure's loss comes back, a scheduler's rate is the one that is used, a scaled loss whose gradients
+    are not finite leaves everything as it was."""
+    from landmark_b200.optim import AdamW
+
+    p = torch.nn.Parameter(torch.ones(300, device="cuda"))
+    opt = AdamW([p], lr=0.5, weight_decay=0.0)
+    rate = torch.optim.lr_scheduler.StepLR(opt, step_size=1, gamma=0.5)
+
+    def closure():
+        opt.zero_grad()
+        loss = p.sum()
+        loss.backward()
+        return loss
+
+    assert float(opt.step(closure).detach()) == 300.0
+    assert float((p.detach() - 0.5).abs().max()) <= 20 * U  # equal gradients: a step is the rate
+    rate.step()
+    opt.step(closure)
+    assert float((p.detach() - 0.25).abs().max()) <= 20 * U
+    scaler = torch.amp.GradScaler("cuda", init_scale=2.0 ** 16)
+    kept = p.detach().clone(), opt.state[p]["step"]
+    opt.zero_grad()
+    scaler.scale((p * float("inf")).sum()).backward()
+    scaler.step(opt)
+    scaler.update()
+    assert torch.equal(p, kept[0]) and opt.state[p]["step"] == kept[1]
+    opt.zero_grad()
+    scaler.scale(p.sum()).backward()
+    scaler.step(opt)
+    assert opt.state[p]["step"] == kept[1] + 1 and not torch.equal(p, kept[0])
+
+
 def test_memory_that_moved_and_captures_are_refused():
     from landmark_b200.optim import AdamWTensors
 
