@@ -465,9 +465,20 @@ typedef struct GnrAdamwTensor {
  *   m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2,
  *   p = p (1 - lr weight_decay) - lr / (1 - beta1^step) m / (sqrt(v / (1 - beta2^step)) + eps),
  * in fp32.  ``state_bits`` 32 or 8; ``step`` counts from 1.  ``tensors_h`` is read before the call returns; a launch that is
- * captured into a CUDA graph repeats this call's addresses, count and rates. */
+ * captured into a CUDA graph repeats this call's addresses, count and rates (the clocked form below does not). */
 int gnr_adamw_step(const GnrAdamwTensor* tensors_h, int n_tensors, int param_type, int grad_type, int state_bits, int64_t step,
                    double lr, double beta1, double beta2, double eps, double weight_decay, uint32_t seed, void* stream);
+
+/* The same with count and rates in device memory (a clock: GNR_ADAMW_CLOCK_BYTES on an 8-byte boundary), for steps that are captured
+ * into a CUDA graph.  gnr_adamw_clock_set: the steps done so far (the next is ``step`` + 1; -1: count and seed stay as they are) and
+ * the rates, enqueued like a copy; gnr_adamw_clock_advance: one step further, once before the step's tensors; gnr_adamw_step_clocked: the step that the
+ * clock stands at. */
+enum { GNR_ADAMW_CLOCK_BYTES = 256 };
+int gnr_adamw_clock_set(void* clock, int64_t step, double lr, double beta1, double beta2, double eps, double weight_decay,
+                        uint32_t seed, void* stream);
+int gnr_adamw_clock_advance(void* clock, void* stream);
+int gnr_adamw_step_clocked(const GnrAdamwTensor* tensors_h, int n_tensors, int param_type, int grad_type, int state_bits,
+                           const void* clock, void* stream);
 
 /* Per-stage timing with CUDA events recorded on the launching stream around every stage of
  * gnr_render_chunk / gnr_render_host (the counterpart of the reference's PipeStagesProfiler,

@@ -15,6 +15,7 @@ LIB_PATH = os.path.join(_PKG, "libgridnerf_b200.so")
 STAGE_NAMES = ("sample", "compact", "density", "weights", "compact_app", "app_gather", "mlp", "composite")
 FP32, FP16, BF16 = 0, 1, 2  # element types of the training entries
 ADAMW_BLOCK = 256  # GNR_ADAMW_BLOCK
+ADAMW_CLOCK_BYTES = 256  # GNR_ADAMW_CLOCK_BYTES
 SAMPLE_STATIC_SCRATCH_BYTES = (4 << 20) + 4096
 MAX_LANES = 8  # GNR_MAX_LANES
 EXPIRE_ANY, EXPIRE_PROJECTION, EXPIRE_NETWORK = 1, 2, 3  # gnr_debug_wait
@@ -130,6 +131,9 @@ SIGNATURES = {
     "gnr_embedding_grad": (_INT, [_P, _INT, _INT, _I64, _P, _INT, _I64, _I64, _I64, C.c_float, _INT, _P, _INT, _I64, _P, _SZ, _P]),
     "gnr_adamw_step": (_INT, [_P, _INT, _INT, _INT, _INT, _I64, C.c_double, C.c_double, C.c_double, C.c_double, C.c_double,
                               C.c_uint32, _P]),
+    "gnr_adamw_clock_set": (_INT, [_P, _I64, C.c_double, C.c_double, C.c_double, C.c_double, C.c_double, C.c_uint32, _P]),
+    "gnr_adamw_clock_advance": (_INT, [_P, _P]),
+    "gnr_adamw_step_clocked": (_INT, [_P, _INT, _INT, _INT, _INT, _P, _P]),
     "gnr_profile_enable": (_INT, [_P, _INT]),
     "gnr_profile_collect": (_INT, [_P, C.POINTER(C.c_float), C.POINTER(C.c_int64)]),
     "gnr_measure_l1_bandwidth": (_INT, [_INT, _INT, C.POINTER(C.c_float)]),

@@ -19,6 +19,8 @@
 #include <math.h>
 #include <string.h>
 
+#include <algorithm>
+
 #include "gnr_internal.cuh"
 #include "gnr_types.cuh"
 
@@ -57,6 +59,17 @@ struct Hyper {
   Twice minus_one, two, eighth;
 };
 
+// Rates and count of steps in device memory, for steps that are captured into a CUDA graph: every replay advances them.
+struct Clock {
+  Hyper h;
+  uint32_t of_step;  // what the tensors' random bits begin with
+  uint32_t seed;
+  int64_t step;
+  double lr, beta1, beta2, eps, decay;
+  double power1, power2;  // betas to the power of step
+};
+static_assert(sizeof(Clock) <= GNR_ADAMW_CLOCK_BYTES, "clock");
+
 template <int K> struct Table {
   Hyper h;
   int n;
@@ -74,6 +87,65 @@ __host__ __device__ __forceinline__ uint32_t hash32(uint32_t i, uint32_t seed) {
   x ^= x >> 15;
   x *= 0xBB67AE85u;
   return x ^ (x >> 16);
+}
+
+__host__ __device__ __forceinline__ Twice twice(double x) { return {(float)x, (float)x}; }
+
+// The numbers of a step from its rates and the betas' powers.  Before the first step: no step.
+__host__ __device__ __forceinline__ Hyper hyper_of(double lr, double beta1, double beta2, double eps, double decay, double power1, double power2, bool first) {
+  Hyper h;
+  h.b1 = twice(beta1);
+  h.b1c = twice(1.0 - beta1);
+  h.b2 = twice(beta2);
+  h.b2c = twice(1.0 - beta2);
+  h.keep = twice(1.0 - lr * decay);
+  h.rate = twice(first ? 0.0 : -lr / (1.0 - power1));
+  h.c2_inv = twice(first ? 1.0 : 1.0 / sqrt(1.0 - power2));
+  h.eps = twice(eps);
+  h.minus_one = twice(-1.0);
+  h.two = twice(2.0);
+  h.eighth = twice(0.125);
+  return h;
+}
+
+__host__ __device__ __forceinline__ uint32_t hash_of_step(int64_t step, uint32_t seed) {
+  return hash32((uint32_t)step, seed + (uint32_t)((uint64_t)step >> 32) * 0xBB67AE85u);
+}
+
+// (a negative step: the clock's own count stays)
+__global__ void adamw_set_clock_kernel(Clock* clock, Clock to) {
+  if (to.step < 0) {
+    to.step = clock->step;
+    to.seed = clock->seed;
+    to.of_step = clock->of_step;
+    to.power1 = pow(to.beta1, (double)to.step);
+    to.power2 = pow(to.beta2, (double)to.step);
+    to.h = hyper_of(to.lr, to.beta1, to.beta2, to.eps, to.decay, to.power1, to.power2, to.step == 0);
+  }
+  *clock = to;
+}
+
+__global__ void adamw_advance_clock_kernel(Clock* clock) {
+  Clock c = *clock;
+  ++c.step;
+  c.power1 *= c.beta1;
+  c.power2 *= c.beta2;
+  c.h = hyper_of(c.lr, c.beta1, c.beta2, c.eps, c.decay, c.power1, c.power2, false);
+  c.of_step = hash_of_step(c.step, c.seed);
+  *clock = c;
+}
+
+// A step's numbers: the kernel's arguments, or (Clocked) the clock's, brought to shared memory by all threads of the block.
+template <bool Clocked, int K> __device__ __forceinline__ const Hyper& hyper_for(const Table<K>& table, const Clock* clock) {
+  if constexpr (Clocked) {
+    __shared__ Hyper s_h;
+    constexpr int kWords = sizeof(Hyper) / 4;
+    if (threadIdx.x < kWords) reinterpret_cast<uint32_t*>(&s_h)[threadIdx.x] = reinterpret_cast<const uint32_t*>(&clock->h)[threadIdx.x];
+    __syncthreads();
+    return s_h;
+  } else {
+    return table.h;
+  }
 }
 
 // Two fp32 numbers in one operation of the packed fp32 instructions: each half rounded as the single operation rounds it.
@@ -178,9 +250,9 @@ template <typename P, typename G, bool Master> __device__ __forceinline__ bool a
 
 // Bound by HBM: 16 values of every array in flight a thread; 335M fp32 values with gradients take 1355 us, 6.9 TB/s (with divisions for the two
 // quotients 1517 us), 60M bf16 values with fp32 copies in 300 tensors 250 us, 6.7 TB/s.
-template <typename P, typename G, bool Master, int K>
-__global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__ Table<K> table) {
-  const Hyper& h = table.h;
+template <typename P, typename G, bool Master, bool Clocked, int K>
+__global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__ Table<K> table, const Clock* __restrict__ clock) {
+  const Hyper& h = hyper_for<Clocked>(table, clock);
   const int number = find_tensor(table);
   const Tensor& t = table.t[number];
   const int64_t begin = (int64_t)(blockIdx.x - table.first[number]) * kChunk;
@@ -468,9 +540,9 @@ template <typename P, typename G, bool Master> struct Chunk8 {
 // cap holds the clock at 1.65 to 1.75 GHz.  Five thread blocks to an SM hide the loads better than a longer run of blocks with the
 // next one's loads ahead of the work (1058 against 948 us on zeros), six spill (1000).  A root by Newton's step from the quick reciprocal
 // root, with a way out for its range, takes as long (954 us), in a pass of its own longer (1091).
-template <typename P, typename G, bool Master, int K>
-__global__ void __launch_bounds__(kThreads8, 5) adamw_8bit_kernel(const __grid_constant__ Table<K> table) {
-  const Hyper& h = table.h;
+template <typename P, typename G, bool Master, bool Clocked, int K>
+__global__ void __launch_bounds__(kThreads8, Clocked ? 4 : 5) adamw_8bit_kernel(const __grid_constant__ Table<K> table, const Clock* __restrict__ clock) {
+  const Hyper& h = hyper_for<Clocked>(table, clock);
   const int number = find_tensor(table);
   const Tensor& t = table.t[number];
   const int64_t first = (int64_t)(blockIdx.x - table.first[number]) * kChunk8;
@@ -484,7 +556,7 @@ __global__ void __launch_bounds__(kThreads8, 5) adamw_8bit_kernel(const __grid_c
   c.master_at = Master ? t.master + first : nullptr;
   c.left = (int)min((int64_t)kChunk8, t.n - first);
   c.place = (uint32_t)first;
-  c.seed = t.seed + (uint32_t)(first >> 32) * 0xBB67AE85u;
+  c.seed = (Clocked ? hash32(t.seed, clock->of_step) : t.seed) + (uint32_t)(first >> 32) * 0xBB67AE85u;
   const int lane = threadIdx.x & 31;
   const int at = (threadIdx.x >> 5) * kBlock;
   if (at >= c.left) return;
@@ -492,15 +564,16 @@ __global__ void __launch_bounds__(kThreads8, 5) adamw_8bit_kernel(const __grid_c
   else c.template step<false>(h, c.template fetch<false>(at + lane * 4), at + lane * 4);
 }
 
-template <int K> int launch_table(const Table<K>& table, uint32_t blocks, int p_type, int g_type, bool master, int bits, cudaStream_t st) {
+template <bool Clocked, int K>
+int launch_table(const Table<K>& table, const Clock* clock, uint32_t blocks, int p_type, int g_type, bool master, int bits, cudaStream_t st) {
   return gnr_with_type(p_type, [&](auto p) {
     return gnr_with_type(g_type, [&](auto g) {
       using P = decltype(p);
       using G = decltype(g);
       auto go = [&](auto has) {
         constexpr bool M = decltype(has)::value && sizeof(P) == 2;
-        if (bits == 8) adamw_8bit_kernel<P, G, M, K><<<blocks, kThreads8, 0, st>>>(table);
-        else adamw_kernel<P, G, M, K><<<blocks, kThreads, 0, st>>>(table);
+        if (bits == 8) adamw_8bit_kernel<P, G, M, Clocked, K><<<blocks, kThreads8, 0, st>>>(table, clock);
+        else adamw_kernel<P, G, M, Clocked, K><<<blocks, kThreads, 0, st>>>(table, clock);
       };
       if (master) go(std::true_type());
       else go(std::false_type());
@@ -510,8 +583,9 @@ template <int K> int launch_table(const Table<K>& table, uint32_t blocks, int p_
   });
 }
 
-template <int K>
-int step_all(const GnrAdamwTensor* tensors, int n, const Hyper& h, int p_type, int g_type, bool master, int bits, uint32_t seed, cudaStream_t st) {
+// (`clock`: null, or where the step's numbers are instead of in `h` and `seed`)
+template <bool Clocked, int K>
+int step_all(const GnrAdamwTensor* tensors, int n, const Hyper& h, const Clock* clock, int p_type, int g_type, int bits, uint32_t seed, cudaStream_t st) {
   const int chunk = bits == 8 ? kChunk8 : kChunk;
   Table<K> table;
   table.h = h;
@@ -526,59 +600,97 @@ int step_all(const GnrAdamwTensor* tensors, int n, const Hyper& h, int p_type, i
       if (blocks + need > 0x7fffffff) break;
       table.first[table.n] = (uint32_t)blocks;
       table.t[table.n++] = {t.param, t.grad, t.exp_avg, t.exp_avg_sq, t.exp_avg_scale, t.exp_avg_sq_scale, t.master, t.n,
-                            hash32((uint32_t)t.number, seed)};
+                            Clocked ? (uint32_t)t.number : hash32((uint32_t)t.number, seed)};
       blocks += need;
     }
     if (table.n > 0)
-      if (int rc = launch_table(table, (uint32_t)blocks, p_type, g_type, master, bits, st)) return rc;
+      if (int rc = launch_table<Clocked>(table, clock, (uint32_t)blocks, p_type, g_type, tensors[0].master != nullptr, bits, st)) return rc;
   }
   return 0;
+}
+
+int check_tensors(const char* what, const GnrAdamwTensor* tensors, int n, int param_type, int grad_type, int bits) {
+  if (n < 0 || (n > 0 && !tensors) || gnr_type_size(param_type) == 0 || gnr_type_size(grad_type) == 0 || (bits != 8 && bits != 32)) {
+    gnr_set_error("%s: null pointer, unknown element type, or states of %d bits (8 or 32)", what, bits);
+    return -1;
+  }
+  const bool master = n > 0 && tensors[0].master != nullptr;
+  if (master && param_type == GNR_FP32) {
+    gnr_set_error("%s: fp32 parameters have no 32-bit copy", what);
+    return -1;
+  }
+  for (int k = 0; k < n; ++k) {
+    const GnrAdamwTensor& t = tensors[k];
+    if (t.n < 0 || t.n > (int64_t)0x7fffffff * (bits == 8 ? kChunk8 : kChunk) ||
+        (t.n > 0 && (!t.param || !t.grad || !t.exp_avg || !t.exp_avg_sq || (bits == 8 && (!t.exp_avg_scale || !t.exp_avg_sq_scale)))) ||
+        (t.master != nullptr) != master) {
+      gnr_set_error("%s: tensor %d of %lld values: null pointer, or some tensors have a 32-bit copy and others none", what, k, (long long)t.n);
+      return -1;
+    }
+  }
+  return 0;
+}
+
+int check_rates(const char* what, int64_t step, int64_t least, double lr, double beta1, double beta2, double eps, double weight_decay) {
+  if (step < least || !(lr >= 0.0) || !(beta1 >= 0.0 && beta1 < 1.0) || !(beta2 >= 0.0 && beta2 < 1.0) || !(eps >= 1e-30) || !(weight_decay >= 0.0) ||
+      !isfinite(lr) || !isfinite(eps) || !isfinite(weight_decay)) {
+    gnr_set_error("%s: step %lld (from %lld), lr %g, betas %g %g ([0, 1)), eps %g (at least 1e-30), weight decay %g", what, (long long)step, (long long)least,
+                  lr, beta1, beta2, eps, weight_decay);
+    return -1;
+  }
+  return 0;
+}
+
+int check_clock(const char* what, const void* clock) {
+  if (clock && (uintptr_t)clock % 8 == 0) return 0;
+  gnr_set_error("%s: the clock is %d bytes of device memory on an 8-byte boundary", what, GNR_ADAMW_CLOCK_BYTES);
+  return -1;
 }
 
 }  // namespace
 
 extern "C" int gnr_adamw_step(const GnrAdamwTensor* tensors_h, int n_tensors, int param_type, int grad_type, int state_bits, int64_t step,
                               double lr, double beta1, double beta2, double eps, double weight_decay, uint32_t seed, void* stream) {
-  if (n_tensors < 0 || (n_tensors > 0 && !tensors_h) || gnr_type_size(param_type) == 0 || gnr_type_size(grad_type) == 0 ||
-      (state_bits != 8 && state_bits != 32)) {
-    gnr_set_error("gnr_adamw_step: null pointer, unknown element type, or states of %d bits (8 or 32)", state_bits);
-    return -1;
-  }
-  if (step < 1 || !(lr >= 0.0) || !(beta1 >= 0.0 && beta1 < 1.0) || !(beta2 >= 0.0 && beta2 < 1.0) || !(eps >= 1e-30) || !(weight_decay >= 0.0) ||
-      !isfinite(lr) || !isfinite(eps) || !isfinite(weight_decay)) {
-    gnr_set_error("gnr_adamw_step: step %lld (from 1), lr %g, betas %g %g ([0, 1)), eps %g (at least 1e-30), weight decay %g",
-                  (long long)step, lr, beta1, beta2, eps, weight_decay);
-    return -1;
-  }
-  const bool master = n_tensors > 0 && tensors_h[0].master != nullptr;
-  if (master && param_type == GNR_FP32) {
-    gnr_set_error("gnr_adamw_step: fp32 parameters have no 32-bit copy");
-    return -1;
-  }
-  for (int k = 0; k < n_tensors; ++k) {
-    const GnrAdamwTensor& t = tensors_h[k];
-    if (t.n < 0 || t.n > (int64_t)0x7fffffff * (state_bits == 8 ? kChunk8 : kChunk) ||
-        (t.n > 0 && (!t.param || !t.grad || !t.exp_avg || !t.exp_avg_sq || (state_bits == 8 && (!t.exp_avg_scale || !t.exp_avg_sq_scale)))) ||
-        (t.master != nullptr) != master) {
-      gnr_set_error("gnr_adamw_step: tensor %d of %lld values: null pointer, or some tensors have a 32-bit copy and others none", k, (long long)t.n);
-      return -1;
-    }
-  }
-  Hyper h;
-  auto twice = [](double x) { return Twice{(float)x, (float)x}; };
-  h.b1 = twice(beta1);
-  h.b1c = twice(1.0 - beta1);
-  h.b2 = twice(beta2);
-  h.b2c = twice(1.0 - beta2);
-  h.keep = twice(1.0 - lr * weight_decay);
-  h.rate = twice(-lr / (1.0 - pow(beta1, (double)step)));
-  h.c2_inv = twice(1.0 / sqrt(1.0 - pow(beta2, (double)step)));
-  h.eps = twice(eps);
-  h.minus_one = twice(-1.0);
-  h.two = twice(2.0);
-  h.eighth = twice(0.125);
-  const uint32_t of_step = hash32((uint32_t)step, seed + (uint32_t)((uint64_t)step >> 32) * 0xBB67AE85u);
+  if (int rc = check_tensors("gnr_adamw_step", tensors_h, n_tensors, param_type, grad_type, state_bits)) return rc;
+  if (int rc = check_rates("gnr_adamw_step", step, 1, lr, beta1, beta2, eps, weight_decay)) return rc;
+  const Hyper h = hyper_of(lr, beta1, beta2, eps, weight_decay, pow(beta1, (double)step), pow(beta2, (double)step), false);
+  const uint32_t of_step = hash_of_step(step, seed);
   const cudaStream_t st = (cudaStream_t)stream;
-  return n_tensors <= kSmall ? step_all<kSmall>(tensors_h, n_tensors, h, param_type, grad_type, master, state_bits, of_step, st)
-                             : step_all<kLarge>(tensors_h, n_tensors, h, param_type, grad_type, master, state_bits, of_step, st);
+  return n_tensors <= kSmall ? step_all<false, kSmall>(tensors_h, n_tensors, h, nullptr, param_type, grad_type, state_bits, of_step, st)
+                             : step_all<false, kLarge>(tensors_h, n_tensors, h, nullptr, param_type, grad_type, state_bits, of_step, st);
+}
+
+extern "C" int gnr_adamw_clock_set(void* clock, int64_t step, double lr, double beta1, double beta2, double eps, double weight_decay, uint32_t seed,
+                                   void* stream) {
+  if (int rc = check_clock("gnr_adamw_clock_set", clock)) return rc;
+  if (int rc = check_rates("gnr_adamw_clock_set", step, -1, lr, beta1, beta2, eps, weight_decay)) return rc;
+  Clock c{};
+  c.power1 = pow(beta1, (double)std::max<int64_t>(step, 0));
+  c.power2 = pow(beta2, (double)std::max<int64_t>(step, 0));
+  c.h = hyper_of(lr, beta1, beta2, eps, weight_decay, c.power1, c.power2, step <= 0);
+  c.of_step = hash_of_step(step, seed);
+  c.seed = seed;
+  c.step = step;
+  c.lr = lr;
+  c.beta1 = beta1;
+  c.beta2 = beta2;
+  c.eps = eps;
+  c.decay = weight_decay;
+  adamw_set_clock_kernel<<<1, 1, 0, (cudaStream_t)stream>>>((Clock*)clock, c);
+  GNR_CUDA_OK(cudaGetLastError());
+  return 0;
+}
+
+extern "C" int gnr_adamw_clock_advance(void* clock, void* stream) {
+  if (int rc = check_clock("gnr_adamw_clock_advance", clock)) return rc;
+  adamw_advance_clock_kernel<<<1, 1, 0, (cudaStream_t)stream>>>((Clock*)clock);
+  GNR_CUDA_OK(cudaGetLastError());
+  return 0;
+}
+
+extern "C" int gnr_adamw_step_clocked(const GnrAdamwTensor* tensors_h, int n_tensors, int param_type, int grad_type, int state_bits, const void* clock,
+                                      void* stream) {
+  if (int rc = check_tensors("gnr_adamw_step_clocked", tensors_h, n_tensors, param_type, grad_type, state_bits)) return rc;
+  if (int rc = check_clock("gnr_adamw_step_clocked", clock)) return rc;
+  return step_all<true, kLarge>(tensors_h, n_tensors, Hyper{}, (const Clock*)clock, param_type, grad_type, state_bits, 0, (cudaStream_t)stream);
 }

@@ -102,34 +102,50 @@ class AdamWTensors:
              weight_decay: float = 1e-2, seed: int = 0):
         """One step with the gradients ``grads`` (of one type, float32 or 16 bits; None leaves its tensor as it is); ``step``
         counts from 1.  ``seed``: of the random rounding of 8-bit states."""
+        table, kind, kept = self._filled(grads)
+        if kind is None:
+            return
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("an AdamW step cannot be captured into a CUDA graph: a replay would repeat this step's count and rates.  Capture "
+                               "step_clocked() with an AdamWClock")
+        index = self.device.index
+        with _on(index):
+            check(lib.gnr_adamw_step(table, len(self.sizes), _TYPES[self.dtype], _TYPES[kind], self.state_bits, step, lr, betas[0], betas[1],
+                                     eps, weight_decay, seed & 0xFFFFFFFF, _raw_stream(index)), "gnr_adamw_step")
+
+    def step_clocked(self, grads: Sequence[Optional[torch.Tensor]], clock: "AdamWClock"):
+        """The step that ``clock`` stands at, for capture into a CUDA graph: replays read the gradients where they lay then."""
+        if clock.device != self.device:
+            raise ValueError(f"clock on {clock.device}, parameters on {self.device}")
+        table, kind, kept = self._filled(grads)
+        if kind is None:
+            return
+        index = self.device.index
+        with _on(index):
+            check(lib.gnr_adamw_step_clocked(table, len(self.sizes), _TYPES[self.dtype], _TYPES[kind], self.state_bits, clock.memory.data_ptr(),
+                                             _raw_stream(index)), "gnr_adamw_step_clocked")
+
+    def _filled(self, grads):
+        """(a copy of the table with the gradients in it, their type or None where there are none, what has to stay until the launch)"""
         if len(grads) != len(self.sizes):
             raise ValueError(f"{len(grads)} gradients for {len(self.sizes)} tensors")
         if list(map(_address, self.params)) != self.starts:
             raise ValueError("a parameter has been given other memory since it was checked")
-        index = self.device.index
-        table = self._words.from_buffer_copy(self._table)  # a copy for this call
+        table = self._words.from_buffer_copy(self._table)
         try:  # all there and as they should be
             kinds = {g.dtype for g in grads}
-            plain = (list(map(_numel, grads)) == self.sizes and set(map(_get_device, grads)) == {index} and len(kinds) == 1
-                     and all(map(_is_contiguous, grads)) and kinds <= _TYPES.keys())
-            if plain and len(grads) > 32:
-                np.frombuffer(table, dtype=np.int64)[_GRAD::_WORDS] = list(map(_address, grads))
-            elif plain:
-                for at, address in zip(range(_GRAD, len(table), _WORDS), map(_address, grads)):
-                    table[at] = address
+            if (list(map(_numel, grads)) == self.sizes and set(map(_get_device, grads)) == {self.device.index} and len(kinds) == 1
+                    and all(map(_is_contiguous, grads)) and kinds <= _TYPES.keys()):
+                if len(grads) > 32:
+                    np.frombuffer(table, dtype=np.int64)[_GRAD::_WORDS] = list(map(_address, grads))
+                else:
+                    for at, address in zip(range(_GRAD, len(table), _WORDS), map(_address, grads)):
+                        table[at] = address
+                return table, kinds.pop(), grads
         except (AttributeError, TypeError, RuntimeError):
-            plain = False
-        if plain:
-            (kind,) = kinds
-        else:
-            grads, kind = self._grads(grads, table)
-            if kind is None:
-                return
-        if torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("an AdamW step cannot be captured into a CUDA graph: a replay would repeat this step's count and rates")
-        with _on(index):
-            check(lib.gnr_adamw_step(table, len(self.sizes), _TYPES[self.dtype], _TYPES[kind], self.state_bits, step, lr, betas[0], betas[1],
-                                     eps, weight_decay, seed & 0xFFFFFFFF, _raw_stream(index)), "gnr_adamw_step")
+            pass
+        kept, kind = self._grads(grads, table)
+        return table, kind, kept
 
     def _grads(self, grads, table):
         """Gradients one by one: some missing, not contiguous or wrong.  Returns what has to stay until the launch, and their type."""
@@ -148,6 +164,39 @@ class AdamWTensors:
             kept.append(g)
             table[k * _WORDS + _GRAD] = g.data_ptr()
         return kept, kind
+
+
+class AdamWClock:
+    """Rates and count of steps on the device, for steps that are captured into a CUDA graph: capture ``advance()`` and one
+    ``AdamWTensors.step_clocked(grads, clock)`` for every set of tensors; every replay is then the next step.  ``set`` changes rates (and the
+    count) between replays, in the order of the stream it is called on."""
+
+    def __init__(self, device, *, lr: float, betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2, step: int = 0,
+                 seed: int = 0):
+        self.memory = torch.zeros(_lib.ADAMW_CLOCK_BYTES, dtype=torch.uint8, device=device)
+        self.device = self.memory.device
+        if self.device.type != "cuda":
+            raise ValueError(f"the clock must be on a CUDA device, got {self.device}")
+        self._rates = {"lr": lr, "betas": tuple(betas), "eps": eps, "weight_decay": weight_decay}
+        self._seed = seed & 0xFFFFFFFF
+        self.set(step=step)
+
+    def set(self, *, step: Optional[int] = None, **rates):
+        """New ``lr``, ``betas``, ``eps`` or ``weight_decay``; ``step``: the steps done so far (None: as many as there are)."""
+        if rates.keys() - self._rates.keys():
+            raise TypeError(f"a clock has {', '.join(self._rates)}, got {', '.join(rates)}")
+        if step is not None and step < 0:
+            raise ValueError(f"step {step}")
+        new = {**self._rates, **rates}
+        with _on(self.device.index):
+            check(lib.gnr_adamw_clock_set(self.memory.data_ptr(), -1 if step is None else step, new["lr"], new["betas"][0], new["betas"][1], new["eps"],
+                                          new["weight_decay"], self._seed, _raw_stream(self.device.index)), "gnr_adamw_clock_set")
+        self._rates = new
+
+    def advance(self):
+        """One step further; once before the ``step_clocked`` calls of a step."""
+        with _on(self.device.index):
+            check(lib.gnr_adamw_clock_advance(self.memory.data_ptr(), _raw_stream(self.device.index)), "gnr_adamw_clock_advance")
 
 
 def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step: int, lr: float, betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,

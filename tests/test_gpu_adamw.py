@@ -380,6 +380,77 @@ def test_closures_schedulers_and_loss_scaling():
     assert opt.state[p]["step"] == kept[1] + 1 and not torch.equal(p, kept[0])
 
 
+@pytest.mark.parametrize("dtype,grad,master", [MIXES[0], MIXES[2], MIXES[6]])
+@pytest.mark.parametrize("eight", [False, True])
+def test_clocked_steps(dtype, grad, master, eight):
+    """Steps by a clock are the steps by number: the same states bit for bit, parameters within the bound of one step each (the betas'
+    powers are running products there)."""
+    from landmark_b200.optim import AdamWClock, AdamWTensors
+
+    def build():
+        p, g, m, v, x = tensors(SIZES, dtype, grad)
+        scales = ()
+        if eight:
+            m, v, *scales = random_states(SIZES)
+        x = x if master else None
+        return AdamWTensors(p, m, v, *(scales or (None, None)), x), g, (p, m, v)
+
+    plain, g, a = build()
+    clocked, g2, b = build()
+    clock = AdamWClock("cuda", lr=1e-2, betas=(0.9, 0.99), weight_decay=0.1, step=5, seed=77)
+    grads = [None if k == 3 else t for k, t in enumerate(g)]
+    for step in range(6, 12):
+        plain.step(grads, step=step, lr=1e-2 if step < 9 else 3e-3, betas=(0.9, 0.99), weight_decay=0.1, seed=77)
+        if step == 9:
+            clock.set(lr=3e-3)
+        clock.advance()
+        clocked.step_clocked([None if k == 3 else t for k, t in enumerate(g2)], clock)
+        for x, y in zip(a[1] + a[2], b[1] + b[2]):
+            assert torch.equal(bits(x), bits(y))
+        off = torch.finfo(dtype).eps * (step - 5)  # a rounding that falls the other way, once a step
+        assert all(bool(((x.float() - y.float()).abs() <= off * (x.float().abs() + 0.1)).all()) for x, y in zip(a[0], b[0]))
+
+
+@pytest.mark.parametrize("eight", [False, True])
+def test_captured_steps_go_on(eight):
+    from landmark_b200.optim import AdamWClock, AdamWTensors
+
+    def build():
+        p, g, m, v, _ = tensors(SIZES, torch.float32, torch.float32)
+        scales = ()
+        if eight:
+            m, v, *scales = random_states(SIZES)
+        return AdamWTensors(p, m, v, *scales), g, (p, m, v)
+
+    eager, g, a = build()
+    graphed, g2, b = build()
+    clocks = [AdamWClock("cuda", lr=1e-2, seed=3) for _ in range(2)]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        clocks[1].advance()
+        graphed.step_clocked(g2, clocks[1])
+    for k in range(8):
+        for x, y in zip(g, g2):
+            x.normal_(0, 1e-3)
+            y.copy_(x)
+        if k == 4:
+            clocks[0].set(lr=1e-3, betas=(0.8, 0.95))
+            clocks[1].set(lr=1e-3, betas=(0.8, 0.95))
+        if k == 6:
+            clocks[0].set(step=1000)
+            clocks[1].set(step=1000)
+        clocks[0].advance()
+        eager.step_clocked(g, clocks[0])
+        graph.replay()
+        for xs, ys in zip(a, b):
+            assert all(torch.equal(bits(x), bits(y)) for x, y in zip(xs, ys))
+    assert torch.equal(clocks[0].memory, clocks[1].memory)
+    for bad in ({"lr": -1.0}, {"betas": (1.0, 0.9)}, {"eps": 0.0}, {"step": -2}, {"rate": 1.0}):
+        with pytest.raises((RuntimeError, TypeError, ValueError)):
+            clocks[0].set(**bad)
+    assert torch.equal(clocks[0].memory, clocks[1].memory)
+
+
 def test_memory_that_moved_and_captures_are_refused():
     from landmark_b200.optim import AdamWTensors
 

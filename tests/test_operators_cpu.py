@@ -66,10 +66,30 @@ def test_adamw_entry_refuses():
     assert _lib.lib.gnr_adamw_step(None, 0, 0, 0, 32, 1, 1e-3, 0.9, 0.999, 1e-8, 0.0, 0, None) == 0
 
 
+def test_clock_entries_refuse():
+    from landmark_b200 import _lib
+
+    lib, p = _lib.lib, C.c_void_p(256)
+    assert lib.gnr_adamw_clock_set(None, 0, 1e-3, 0.9, 0.999, 1e-8, 0.0, 0, None) < 0
+    assert lib.gnr_adamw_clock_set(C.c_void_p(257), 0, 1e-3, 0.9, 0.999, 1e-8, 0.0, 0, None) < 0
+    for bad in ((-2, 1e-3, 0.9, 0.999, 1e-8, 0.0), (0, -1.0, 0.9, 0.999, 1e-8, 0.0), (0, 1e-3, 1.0, 0.999, 1e-8, 0.0), (0, 1e-3, 0.9, 1.0, 1e-8, 0.0),
+                (0, 1e-3, 0.9, 0.999, 0.0, 0.0), (0, 1e-3, 0.9, 0.999, 1e-8, -1.0)):
+        assert lib.gnr_adamw_clock_set(p, *bad, 0, None) < 0, bad
+    assert lib.gnr_adamw_clock_advance(None, None) < 0
+    t = (_lib.GnrAdamwTensor * 1)()
+    assert lib.gnr_adamw_step_clocked(t, 1, 0, 0, 32, None, None) < 0
+    t[0].n = 5
+    assert lib.gnr_adamw_step_clocked(t, 1, 0, 0, 32, p, None) < 0
+    t[0].n = 0
+    assert lib.gnr_adamw_step_clocked(t, 1, 0, 0, 32, p, None) == 0
+
+
 def test_adamw_refuses():
-    from landmark_b200.optim import AdamW, AdamWTensors, state_blocks
+    from landmark_b200.optim import AdamW, AdamWClock, AdamWTensors, state_blocks
 
     x = torch.zeros(4)
+    with pytest.raises(ValueError, match="CUDA"):
+        AdamWClock("cpu", lr=1e-3)
     with pytest.raises(ValueError, match="CUDA"):
         AdamWTensors([x], [x], [x])
     with pytest.raises(TypeError, match="float64"):
