@@ -465,16 +465,25 @@ __device__ __forceinline__ float* piece_at(const SumArgs& a, int64_t block, int 
   return a.pieces + (block * 2 + which) * a.piece_stride + at;
 }
 
-// first position of the sorted keys that is not below `key`, found by a warp
-__device__ __forceinline__ int64_t warp_lower_bound(const uint32_t* keys, int64_t n, uint32_t key) {
+// Which of the answers 0 .. n a search by 32 probes at once finds; `below(lo, hi, step)` counts those of the places lo + step - 1,
+// lo + 2 step - 1, ... lo + 32 step - 1 that lie before `hi` and before the answer.  hi - lo + 1 answers are left, the probes part them
+// into 33 runs of `step`: 33 step has to reach all of them, or the last would be cut off.
+template <typename Below> __device__ __forceinline__ int64_t probed_bound(int64_t n, Below below) {
   int64_t lo = 0, hi = n;
   while (lo < hi) {
-    const int64_t step = (hi - lo + 32) / 33, at = lo + ((threadIdx.x & 31) + 1) * step - 1;
-    const int below = __popc(__ballot_sync(0xffffffffu, at < hi && keys[at] < key));
-    lo += below * step;
-    hi = min(hi, lo + step - 1);
+    const int64_t step = (hi - lo) / 33 + 1;
+    lo += below(lo, hi, step) * step;
+    hi = lo + step - 1 < hi ? lo + step - 1 : hi;
   }
   return lo;
+}
+
+// first position of the sorted keys that is not below `key`, found by a warp
+__device__ __forceinline__ int64_t warp_lower_bound(const uint32_t* keys, int64_t n, uint32_t key) {
+  return probed_bound(n, [&](int64_t lo, int64_t hi, int64_t step) {
+    const int64_t at = lo + ((threadIdx.x & 31) + 1) * step - 1;
+    return __popc(__ballot_sync(0xffffffffu, at < hi && keys[at] < key));
+  });
 }
 
 // zeros in those rows from `first` on that no token names

@@ -332,3 +332,33 @@ def test_offsets_past_32_bits():
     g = torch.ones((t, d), dtype=torch.bfloat16, device="cuda")
     idx = torch.arange(t, device="cuda") % 1000
     assert bool((embedding_backward(g, idx, 1000, dtype=torch.float32) == 1100).all())  # whole numbers: exact in fp32
+
+
+@pytest.mark.parametrize("t", [2049, 2179, 2200, 2211, 2310, 4950, 9009, 33000, 65536, 65537, 100000, 1500007])
+@pytest.mark.parametrize("v,d,dtype", [(0, 1, torch.float32), (0, 48, torch.float32), (0, 5, torch.float16), (131072, 48, torch.bfloat16)])
+def test_every_row_is_named_once(t, v, d, dtype):
+    """No token is masked and no row has two: each row's gradient is its token's row, bit for bit, in every call, and no row that is
+    named is taken for one that is not (its zeros would be written beside its sum)."""
+    from landmark_b200.embedding import embedding_backward
+
+    gen = torch.Generator(device="cuda").manual_seed(t)
+    rows = max(t, v)
+    g = torch.randn((t, d), generator=gen, device="cuda").to(dtype)
+    out = torch.empty((rows, d), dtype=dtype, device="cuda")
+    for idx in (torch.arange(t, device="cuda"), torch.randperm(rows, generator=gen, device="cuda")[:t], torch.arange(rows - t, rows, device="cuda").flip(0)):
+        want = torch.zeros_like(out)
+        want[idx] = g
+        for _ in range(5):
+            assert torch.equal(embedding_backward(g, idx, rows, out=out.fill_(float("nan"))), want)
+
+
+@pytest.mark.parametrize("t", [2200, 2310, 4950, 9009])
+def test_named_rows_of_a_wide_table(t):
+    """Uniform tokens of 2048 values against a table of many more rows: what is marked as named decides most of what is written."""
+    from landmark_b200.embedding import embedding_backward
+
+    idx, g, _ = make(t, 131072, 2048, torch.bfloat16, seed=t)
+    got = embedding_backward(g, idx, 131072)
+    check_gradient(got, g, idx, 131072)
+    for _ in range(5):
+        assert torch.equal(got, embedding_backward(g, idx, 131072))
