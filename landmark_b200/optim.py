@@ -37,6 +37,12 @@ def state_blocks(numel: int) -> int:
     return -(-numel // BLOCK)
 
 
+def _no_capture():
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("an AdamW step cannot be captured into a CUDA graph: a replay would repeat this step's count and rates.  Capture "
+                           "AdamWTensors.step_clocked() with an AdamWClock")
+
+
 class AdamWTensors:
     """Parameters and optimiser states that are stepped together: checked once, then stepped with new gradients.
 
@@ -105,11 +111,9 @@ class AdamWTensors:
         table, kind, kept = self._filled(grads)
         if kind is None:
             return
-        if torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("an AdamW step cannot be captured into a CUDA graph: a replay would repeat this step's count and rates.  Capture "
-                               "step_clocked() with an AdamWClock")
         index = self.device.index
         with _on(index):
+            _no_capture()
             check(lib.gnr_adamw_step(table, len(self.sizes), _TYPES[self.dtype], _TYPES[kind], self.state_bits, step, lr, betas[0], betas[1],
                                      eps, weight_decay, seed & 0xFFFFFFFF, _raw_stream(index)), "gnr_adamw_step")
 
@@ -246,8 +250,14 @@ class AdamW(torch.optim.Optimizer):
         self._sets = {}
 
     def _state_of(self, p: torch.Tensor) -> dict:
-        s = self.state[p]
-        if not s:
+        """The state of ``p``; a new one, not yet entered, where it has none or a part is missing."""
+        s = self.state.get(p)
+        fresh = not s
+        copied = self.master_weights and p.dtype != torch.float32 and (fresh or "master" not in s)
+        if not fresh and not copied:
+            return s
+        s = dict(s or {})
+        if fresh:
             s["step"] = 0
             kind = _CODES if self.state_bits == 8 else torch.float32
             for name in ("exp_avg", "exp_avg_sq"):
@@ -255,7 +265,7 @@ class AdamW(torch.optim.Optimizer):
                 if self.state_bits == 8:
                     s[name] = s[name].view(kind)
                     s[name + "_scale"] = torch.zeros(state_blocks(p.numel()), device=p.device)
-        if self.master_weights and p.dtype != torch.float32 and "master" not in s:
+        if copied:
             s["master"] = p.detach().float()
         return s
 
@@ -272,27 +282,36 @@ class AdamW(torch.optim.Optimizer):
         parts = {n: [s.get(n) for s in states] for n in ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale", "master") if n in states[0]}
         made = AdamWTensors([p.detach() for p in params], parts["exp_avg"], parts["exp_avg_sq"], parts.get("exp_avg_scale"), parts.get("exp_avg_sq_scale"),
                             parts.get("master"))
+        for p, state in zip(params, states):  # (only now: what is refused leaves no state behind)
+            self.state[p] = state
         self._sets[key] = (params, states, parts, made)
         return states, made
 
     @torch.no_grad()
     def step(self, closure=None):
+        if torch.cuda.is_initialized():
+            _no_capture()
         loss = None
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        todo = []  # every set of every group: states are made, and refusals raised, before anything is stepped
         for number, group in enumerate(self.param_groups):
             sets: dict = {}
             for p in group["params"]:
                 if p.grad is not None:
                     sets.setdefault((number, p.device, p.dtype), []).append(p)
             for k, (key, params) in enumerate(sets.items()):
-                states, tensors = self._tensors(key, params)
-                counts = {s["step"] for s in states}
-                for t in sorted(counts):  # one, unless a parameter had no gradient in some steps
-                    grads = [p.grad if len(counts) == 1 or s["step"] == t else None for p, s in zip(params, states)]
-                    tensors.step(grads, step=int(t) + 1, lr=float(group["lr"]), betas=group["betas"], eps=group["eps"],
-                                 weight_decay=group["weight_decay"], seed=self.seed + 0x3C6EF372 * (2 * number + 1) + k)
-                for s in states:
-                    s["step"] += 1
+                if key[1].type == "cuda":
+                    with _on(key[1].index):
+                        _no_capture()
+                todo.append((number, group, k, params, *self._tensors(key, params)))
+        for number, group, k, params, states, tensors in todo:
+            counts = {s["step"] for s in states}
+            for t in sorted(counts):  # one, unless a parameter had no gradient in some steps
+                grads = [p.grad if len(counts) == 1 or s["step"] == t else None for p, s in zip(params, states)]
+                tensors.step(grads, step=int(t) + 1, lr=float(group["lr"]), betas=group["betas"], eps=group["eps"],
+                             weight_decay=group["weight_decay"], seed=self.seed + 0x3C6EF372 * (2 * number + 1) + k)
+            for s in states:
+                s["step"] += 1
         return loss

@@ -492,3 +492,32 @@ def test_offsets_past_32_bits():
     # equal values: every code is the largest one, and the step is the rate
     assert bool((bits(m) == 0x7E).all()) and bool((bits(v) == 0x7E).all())
     assert bool((p == 0.25).all())
+
+
+@pytest.mark.parametrize("state_bits", [8, 32])
+def test_refused_steps_leave_no_state(state_bits):
+    """A first step of the class under a capture is refused before it makes states (their zeros and copies would be captured and never
+    written); the eager step that follows is the formula's first."""
+    from landmark_b200.optim import AdamW
+
+    torch.manual_seed(2)
+    p = [torch.nn.Parameter(torch.randn(n, device="cuda").to(d)) for n, d in ((300, torch.float32), (515, torch.bfloat16))]
+    x = [q.detach().float().clone() for q in p]
+    opt = AdamW(p, lr=1e-2, weight_decay=0.1, state_bits=state_bits)
+    for q in p:
+        q.grad = torch.randn_like(q)
+    calls = []
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="captured"):
+        with torch.cuda.graph(graph):
+            opt.step(lambda: calls.append(1))
+    assert len(opt.state) == 0 and not calls
+    torch.full((1 << 20,), float("nan"), device="cuda")  # what freed memory may hold
+    opt.step()
+    for q, a in zip(p, x):
+        zero = torch.zeros_like(a).double()
+        (want, _, _), (tol, _, _) = reference(a.double(), q.grad.double(), zero, zero, 1, 1e-2, (0.9, 0.999), 1e-8, 0.1)
+        assert opt.state[q]["step"] == 1
+        got = q if q.dtype == torch.float32 else opt.state[q]["master"]
+        assert bool(((got.double() - want).abs() <= tol).all())
+        assert torch.equal(q, got.to(q.dtype))

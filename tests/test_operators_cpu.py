@@ -126,3 +126,15 @@ def test_random_bits_are_even():
         for x in (h, h ^ h.roll(1), h ^ h.roll(256)):
             for b in range(32):
                 assert abs(int(((x >> b) & 1).sum()) - n / 2) <= 6 * (n / 4) ** 0.5
+
+
+def test_adamw_refusals_leave_no_state():
+    from landmark_b200.optim import AdamW
+
+    for dtype in (torch.float32, torch.bfloat16):
+        p = torch.nn.Parameter(torch.zeros(4, dtype=dtype))
+        opt = AdamW([p])
+        p.grad = torch.zeros_like(p)
+        with pytest.raises(ValueError, match="CUDA"):
+            opt.step()
+        assert len(opt.state) == 0 and opt.state_dict()["state"] == {}
