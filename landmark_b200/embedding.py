@@ -16,6 +16,7 @@ import ctypes as C
 from typing import Optional
 
 import torch
+from torch.autograd.graph import increment_version
 
 from . import _lib
 from ._lib import check, lib
@@ -215,4 +216,6 @@ def embedding_backward(grad_output: torch.Tensor, indices: torch.Tensor, num_row
         raise ValueError(f"out must have neighbouring values next to each other and rows that do not overlap, got strides {out.stride()}")
     if torch.is_grad_enabled() and (grad_output.requires_grad or out.requires_grad):
         raise RuntimeError("embedding_backward writes out in place and is not differentiable then")
-    return _gradient(grad_output, indices, float(scale), padding_idx, out, bool(accumulate))
+    _gradient(grad_output, indices, float(scale), padding_idx, out, bool(accumulate))
+    increment_version(out)  # a backward pass over what was computed from the old values is an error
+    return out

@@ -20,6 +20,7 @@ from typing import List, Optional, Sequence, Tuple
 
 import numpy as np
 import torch
+from torch.autograd.graph import increment_version
 
 from . import _lib
 from ._lib import check, lib
@@ -101,8 +102,11 @@ class AdamWTensors:
         self._table[:, _N + 1] = np.arange(len(sizes))
         self.starts = self._table[:, 0].tolist()  # addresses of the parameters
         self._words = C.c_int64 * self._table.size
+        written = [t for tensors, _, _ in self._tensors.values() for t in tensors]
+        # what autograd counts the writes of: views share the count of the tensor that they are views of
+        self._written = list({id(t): t for t in (t if t._base is None else t._base for t in written)}.values())
         # the memory that the table names stays, whatever becomes of the tensors
-        self._kept = [t.detach() for tensors, _, _ in self._tensors.values() for t in tensors]
+        self._kept = [t.detach() for t in written]
 
     def step(self, grads: Sequence[Optional[torch.Tensor]], *, step: int, lr: float, betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
              weight_decay: float = 1e-2, seed: int = 0):
@@ -116,6 +120,7 @@ class AdamWTensors:
             _no_capture()
             check(lib.gnr_adamw_step(table, len(self.sizes), _TYPES[self.dtype], _TYPES[kind], self.state_bits, step, lr, betas[0], betas[1],
                                      eps, weight_decay, seed & 0xFFFFFFFF, _raw_stream(index)), "gnr_adamw_step")
+        self._tell_autograd(None if kept is grads else grads)
 
     def step_clocked(self, grads: Sequence[Optional[torch.Tensor]], clock: "AdamWClock"):
         """The step that ``clock`` stands at, for capture into a CUDA graph: replays read the gradients where they lay then."""
@@ -128,6 +133,15 @@ class AdamWTensors:
         with _on(index):
             check(lib.gnr_adamw_step_clocked(table, len(self.sizes), _TYPES[self.dtype], _TYPES[kind], self.state_bits, clock.memory.data_ptr(),
                                              _raw_stream(index)), "gnr_adamw_step_clocked")
+        self._tell_autograd(None if kept is grads else grads)
+
+    def _tell_autograd(self, grads):
+        """The step's tensors (``grads``: those that have a gradient) have been written: a backward pass over what was computed from them
+        before is an error."""
+        if grads is None:
+            increment_version(self._written)
+        else:
+            increment_version([t for tensors, _, _ in self._tensors.values() for t, g in zip(tensors, grads) if g is not None])
 
     def _filled(self, grads):
         """(a copy of the table with the gradients in it, their type or None where there are none, what has to stay until the launch)"""

@@ -521,3 +521,38 @@ def test_refused_steps_leave_no_state(state_bits):
         got = q if q.dtype == torch.float32 else opt.state[q]["master"]
         assert bool(((got.double() - want).abs() <= tol).all())
         assert torch.equal(q, got.to(q.dtype))
+
+
+@pytest.mark.parametrize("state_bits", [8, 32])
+def test_backward_over_stepped_parameters_is_refused(state_bits):
+    """A second backward pass over a graph that kept a parameter's old values is an error, as with torch's optimisers; a parameter that
+    had no gradient was not written."""
+    from landmark_b200.optim import AdamW, AdamWClock, AdamWTensors
+
+    p = [torch.nn.Parameter(torch.randn(300, device="cuda")) for _ in range(3)]
+    opt = AdamW(p, state_bits=state_bits)
+    losses = [q.square().sum() for q in p]
+    losses[0].backward(retain_graph=True)
+    losses[1].backward(retain_graph=True)
+    opt.step()
+    for loss in losses[:2]:
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+    losses[2].backward()
+    if state_bits == 32:
+        q, g, m, v = ([t.clone() for t in ts] for ts in tensors([100, 50], torch.float32, torch.float32)[:4])  # (views share their base's count)
+        for clocked in (False, True):
+            kept = [t.requires_grad_(True).square().sum() for t in q]
+            with torch.no_grad():
+                made = AdamWTensors(q, m, v)
+                before = [t._version for t in q + m + v]
+                if clocked:
+                    clock = AdamWClock("cuda", lr=1e-3)
+                    clock.advance()
+                    made.step_clocked([g[0], None], clock)
+                else:
+                    made.step([g[0], None], step=1, lr=1e-3)
+                assert [t._version > b for t, b in zip(q + m + v, before)] == [True, False] * 3
+            with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                kept[0].backward()
+            kept[1].backward()

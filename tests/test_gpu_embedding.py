@@ -362,3 +362,15 @@ def test_named_rows_of_a_wide_table(t):
     check_gradient(got, g, idx, 131072)
     for _ in range(5):
         assert torch.equal(got, embedding_backward(g, idx, 131072))
+
+
+@pytest.mark.parametrize("accumulate", [False, True])
+def test_backward_over_a_written_out_is_refused(accumulate):
+    from landmark_b200.embedding import embedding_backward
+
+    idx, g, w = make(300, 40, 48, torch.float32)
+    x = torch.ones((40, 48), device="cuda", requires_grad=True)
+    loss = (w * x).sum()  # keeps w
+    embedding_backward(g, idx, 40, out=w, accumulate=accumulate)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
