@@ -3,7 +3,7 @@
 ``embedding`` looks rows of a table up: the appearance latent of every ray or sample of an ``encode_app`` model
 (``compute_app_latent``, app/models/gridnerf_sequential.py:429-437, does it with one row for all), or any other table's rows.
 ``embedding_backward`` is its gradient and, read the other way, the sum of the rows that share an index: samples into rays.
-Both are differentiable, each being the other's gradient.
+Both are differentiable, each being the other's gradient; forward-mode tangents go through the same operators.
 
 Indices are int32 or int64, of any shape and strides.  A negative one is a masked place: it looks up zeros and adds nothing.
 One that is not below the number of rows looks up NaN and adds nothing (only the device sees it, so no error is raised).
@@ -16,6 +16,7 @@ import ctypes as C
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.graph import increment_version
 
 from . import _lib
@@ -131,10 +132,20 @@ def _no_capture(what: str):
                            "stream of an earlier pass.  Capture embedding() and embedding_backward() themselves, without autograd")
 
 
+def _has_tangent(t: torch.Tensor) -> bool:
+    """Whether forward-mode differentiation goes through ``t`` (asked only inside a dual level, where this torch says so cheaply)."""
+    return getattr(forward_ad, "_current_level", 0) >= 0 and forward_ad.unpack_dual(t).tangent is not None
+
+
+def _differentiated(t: torch.Tensor) -> bool:
+    return (t.requires_grad and torch.is_grad_enabled()) or _has_tangent(t)
+
+
 class _Embedding(torch.autograd.Function):
     @staticmethod
     def forward(ctx, indices, weight, scale, padding_idx):
         ctx.save_for_backward(indices)
+        ctx.save_for_forward(indices)
         ctx.args = weight.shape[0], scale, padding_idx, weight.dtype
         return _lookup(indices, weight, scale)
 
@@ -144,12 +155,18 @@ class _Embedding(torch.autograd.Function):
         rows, scale, padding_idx, dtype = ctx.args
         return None, embedding_backward(grad, ctx.saved_tensors[0], rows, scale=scale, padding_idx=padding_idx, dtype=dtype), None, None
 
+    @staticmethod
+    def jvp(ctx, _, tangent, *rest):  # the lookup is linear in the table
+        return embedding(ctx.saved_tensors[0], tangent, scale=ctx.args[1], padding_idx=ctx.args[2])
+
 
 class _EmbeddingBackward(torch.autograd.Function):
     @staticmethod
     def forward(ctx, grad, indices, num_rows, scale, padding_idx, dtype):
         ctx.save_for_backward(indices)
+        ctx.save_for_forward(indices)
         ctx.args = scale, padding_idx, grad.dtype, grad.shape
+        ctx.result = num_rows, dtype
         return _new_gradient(grad, indices, num_rows, scale, padding_idx, dtype)
 
     @staticmethod
@@ -159,6 +176,11 @@ class _EmbeddingBackward(torch.autograd.Function):
         indices = ctx.saved_tensors[0]
         indices = torch.where((indices == (-1 if padding_idx is None else padding_idx)) | (indices >= grad.shape[0]), -1, indices)
         return embedding(indices, grad, scale=scale).to(dtype).reshape(shape), None, None, None, None, None
+
+    @staticmethod
+    def jvp(ctx, tangent, *rest):  # the sum is linear in what it sums
+        num_rows, dtype = ctx.result
+        return embedding_backward(tangent, ctx.saved_tensors[0], num_rows, scale=ctx.args[0], padding_idx=ctx.args[1], dtype=dtype)
 
 
 def _new_gradient(grad, indices, num_rows, scale, padding_idx, dtype):
@@ -177,7 +199,7 @@ def embedding(indices: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, p
     The product is taken in fp32 and rounded once.  ``padding_idx``: a row that gets no gradient."""
     if padding_idx is not None:
         padding_idx = _check_padding(padding_idx, weight.shape[0])
-    if weight.requires_grad and torch.is_grad_enabled():
+    if _differentiated(weight):
         return _Embedding.apply(indices, weight, float(scale), padding_idx)
     return _lookup(indices, weight, float(scale))
 
@@ -204,7 +226,7 @@ def embedding_backward(grad_output: torch.Tensor, indices: torch.Tensor, num_row
             dtype = grad_output.dtype
         elif dtype not in _TYPES:
             raise TypeError(f"dtype must be float32, float16 or bfloat16, got {dtype}")
-        if grad_output.requires_grad and torch.is_grad_enabled():
+        if _differentiated(grad_output):
             return _EmbeddingBackward.apply(grad_output, indices, num_rows, float(scale), padding_idx, dtype)
         return _new_gradient(grad_output, indices, num_rows, float(scale), padding_idx, dtype)
     _kind("out", out)
@@ -214,7 +236,7 @@ def embedding_backward(grad_output: torch.Tensor, indices: torch.Tensor, num_row
         raise ValueError(f"out {tuple(out.shape)} on {out.device} must be {(num_rows, grad_output.shape[-1])} on {grad_output.device}")
     if (out.stride(1) != 1 and out.shape[1] > 1) or (num_rows > 1 and out.stride(0) < out.shape[1]):
         raise ValueError(f"out must have neighbouring values next to each other and rows that do not overlap, got strides {out.stride()}")
-    if torch.is_grad_enabled() and (grad_output.requires_grad or out.requires_grad):
+    if _differentiated(grad_output) or _differentiated(out):
         raise RuntimeError("embedding_backward writes out in place and is not differentiable then")
     _gradient(grad_output, indices, float(scale), padding_idx, out, bool(accumulate))
     increment_version(out)  # a backward pass over what was computed from the old values is an error

@@ -374,3 +374,37 @@ def test_backward_over_a_written_out_is_refused(accumulate):
     embedding_backward(g, idx, 40, out=w, accumulate=accumulate)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         loss.backward()
+
+
+def test_forward_mode_tangents():
+    """Both operators are linear: the tangent of a result is the operator's result for the tangent, with and without a backward pass as
+    well, and its gradient is the other operator."""
+    import torch.autograd.forward_ad as fwd
+
+    from landmark_b200.embedding import embedding, embedding_backward
+
+    for dtype in (torch.float32, torch.bfloat16):
+        idx, g, w = make(500, 40, 24, dtype, masked=0.2)
+        dw, dg = torch.randn_like(w), torch.randn_like(g)
+        for grad in (False, True):
+            with fwd.dual_level():
+                a, b = w.clone().requires_grad_(grad), g.clone().requires_grad_(grad)
+                da, db = dw.clone().requires_grad_(grad), dg.clone().requires_grad_(grad)
+                out = fwd.unpack_dual(embedding(idx, fwd.make_dual(a, da), scale=0.5, padding_idx=7))
+                assert torch.equal(out.primal, embedding(idx, w, scale=0.5)) and torch.equal(out.tangent, embedding(idx, dw, scale=0.5))
+                total = fwd.unpack_dual(embedding_backward(fwd.make_dual(b, db), idx, 40, scale=0.5, padding_idx=7, dtype=torch.float32))
+                assert torch.equal(total.primal, embedding_backward(g, idx, 40, scale=0.5, padding_idx=7, dtype=torch.float32))
+                assert torch.equal(total.tangent, embedding_backward(dg, idx, 40, scale=0.5, padding_idx=7, dtype=torch.float32))
+                if grad:  # the tangent's own gradient
+                    (got,) = torch.autograd.grad((out.tangent * g).sum(), da)
+                    assert torch.equal(got, embedding_backward(g, idx, 40, scale=0.5, padding_idx=7))
+                into = torch.zeros((40, 24), dtype=dtype, device="cuda")
+                with pytest.raises(RuntimeError, match="not differentiable"):
+                    embedding_backward(fwd.make_dual(g, dg), idx, 40, out=into)
+                with pytest.raises(RuntimeError, match="not differentiable"):
+                    embedding_backward(g, idx, 40, out=fwd.make_dual(into, into.clone()), accumulate=True)
+                plain = fwd.unpack_dual(embedding(idx, w))  # no tangent: none comes out
+                assert plain.tangent is None and torch.equal(plain.primal, embedding(idx, w))
+    with torch.no_grad(), fwd.dual_level():
+        idx, g, w = make(50, 40, 24, torch.float32)
+        assert fwd.unpack_dual(embedding(idx, fwd.make_dual(w, g[:40]))).tangent is not None
