@@ -224,8 +224,18 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step: int, lr: float, be
         grads, step=step, lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, seed=seed)
 
 
+def _check_group(group: dict):
+    """Refuses what torch's optimisers have in their groups and a step here would not do."""
+    for name in ("maximize", "amsgrad", "differentiable"):
+        if group.get(name):
+            raise ValueError(f"{name} is not offered")
+    if group.get("decoupled_weight_decay") is False and group.get("weight_decay", 0):
+        raise ValueError("coupled weight decay (decoupled_weight_decay=False, as of torch.optim.Adam) is not offered")
+
+
 class AdamW(torch.optim.Optimizer):
-    """``torch.optim.AdamW`` over dense CUDA parameters: groups, learning rate schedulers and ``state_dict`` as there.
+    """``torch.optim.AdamW`` over dense CUDA parameters: groups, learning rate schedulers and ``state_dict`` as there.  Groups that
+    ask for ``maximize``, ``amsgrad``, ``differentiable`` or coupled weight decay are refused.
 
     ``state_bits``: 32 or 8.  ``master_weights``: 16-bit parameters keep an fp32 copy in the state.  ``seed``: of the random
     rounding of 8-bit states."""
@@ -241,12 +251,16 @@ class AdamW(torch.optim.Optimizer):
         super().__init__(params, {"lr": lr, "betas": betas, "eps": eps, "weight_decay": weight_decay})
 
     def add_param_group(self, param_group):
+        if isinstance(param_group, dict):  # (what is not is refused by torch)
+            _check_group({**self.defaults, **param_group})
         super().add_param_group(param_group)
         self._sets.clear()
 
     def load_state_dict(self, state_dict):
         """Restores what ``state_dict`` returned, every state in its own type (torch would give it the parameter's).  The state of a
-        ``torch.optim.AdamW`` with fp32 moments is taken as well."""
+        ``torch.optim.AdamW`` (or of an ``Adam`` without weight decay) with fp32 moments is taken as well."""
+        for group in state_dict["param_groups"]:
+            _check_group(group)
         super().load_state_dict(state_dict)
         self._sets.clear()
         saved = state_dict["state"]
@@ -305,6 +319,8 @@ class AdamW(torch.optim.Optimizer):
     def step(self, closure=None):
         if torch.cuda.is_initialized():
             _no_capture()
+        for group in self.param_groups:
+            _check_group(group)
         loss = None
         if closure is not None:
             with torch.enable_grad():

@@ -138,3 +138,42 @@ def test_adamw_refusals_leave_no_state():
         with pytest.raises(ValueError, match="CUDA"):
             opt.step()
         assert len(opt.state) == 0 and opt.state_dict()["state"] == {}
+
+
+def test_adamw_refuses_groups_it_would_not_obey():
+    from landmark_b200.optim import AdamW
+
+    def params():
+        return [torch.nn.Parameter(torch.zeros(4)) for _ in range(2)]
+
+    def state_of(cls, **options):
+        ps = params()
+        opt = cls(ps, lr=0.25, **options)
+        for p in ps:
+            p.grad = torch.ones(4)
+        opt.step()
+        return opt.state_dict()
+
+    bad = [(torch.optim.AdamW, {"maximize": True}), (torch.optim.AdamW, {"amsgrad": True}), (torch.optim.Adam, {"weight_decay": 0.1}),
+           (torch.optim.Adam, {"maximize": True})]
+    for cls, options in bad:
+        opt = AdamW(params(), lr=0.5)
+        with pytest.raises(ValueError, match="not offered"):
+            opt.load_state_dict(state_of(cls, **options))
+        assert opt.param_groups[0]["lr"] == 0.5 and len(opt.state) == 0  # nothing has been replaced
+    for cls, options in ((torch.optim.AdamW, {}), (torch.optim.Adam, {}), (torch.optim.AdamW, {"foreach": True})):
+        opt = AdamW(params(), lr=0.5)
+        opt.load_state_dict(state_of(cls, **options))
+        assert opt.param_groups[0]["lr"] == 0.25 and [s["step"] for s in opt.state.values()] == [1, 1]
+    for name, value in (("maximize", True), ("amsgrad", True), ("differentiable", True), ("decoupled_weight_decay", False)):
+        with pytest.raises(ValueError, match="not offered"):
+            AdamW([{"params": params(), name: value}], weight_decay=0.1)
+        opt = AdamW(params(), weight_decay=0.1)
+        with pytest.raises(ValueError, match="not offered"):
+            opt.add_param_group({"params": params(), name: value})
+        assert len(opt.param_groups) == 1
+        opt.param_groups[0][name] = value
+        with pytest.raises(ValueError, match="not offered"):
+            opt.step()
+    opt = AdamW([{"params": params(), "decoupled_weight_decay": False, "weight_decay": 0.0, "maximize": False}], weight_decay=0.1)
+    opt.step()
