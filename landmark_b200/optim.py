@@ -259,16 +259,27 @@ class AdamW(torch.optim.Optimizer):
     def load_state_dict(self, state_dict):
         """Restores what ``state_dict`` returned, every state in its own type (torch would give it the parameter's).  The state of a
         ``torch.optim.AdamW`` (or of an ``Adam`` without weight decay) with fp32 moments is taken as well."""
-        for group in state_dict["param_groups"]:
-            _check_group(group)
-        super().load_state_dict(state_dict)
-        self._sets.clear()
-        saved = state_dict["state"]
-        ids = [i for group in state_dict["param_groups"] for i in group["params"]]
-        for i, p in zip(ids, [p for group in self.param_groups for p in group["params"]]):
-            if i in saved:
-                self.state[p] = {k: int(v) if k == "step" else v.detach().to(p.device, copy=True) if isinstance(v, torch.Tensor) else v
-                                 for k, v in saved[i].items()}
+        def check(_, loaded):  # the last hook before and the first behind torch's own work: on what the user's hooks made of the dict
+            for group in loaded["param_groups"]:
+                _check_group(group)
+            taken.append(loaded)
+
+        def keep_types(_):
+            self._sets.clear()
+            saved = taken[0]["state"]
+            ids = [i for group in taken[0]["param_groups"] for i in group["params"]]
+            for i, p in zip(ids, [p for group in self.param_groups for p in group["params"]]):
+                if i in saved:
+                    self.state[p] = {k: int(v) if k == "step" else v.detach().to(p.device, copy=True) if isinstance(v, torch.Tensor) else v
+                                     for k, v in saved[i].items()}
+
+        taken: list = []
+        hooks = self.register_load_state_dict_pre_hook(check), self.register_load_state_dict_post_hook(keep_types, prepend=True)
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            for hook in hooks:
+                hook.remove()
 
     def __getstate__(self):
         return {**super().__getstate__(), "state_bits": self.state_bits, "master_weights": self.master_weights, "seed": self.seed}

@@ -177,3 +177,37 @@ def test_adamw_refuses_groups_it_would_not_obey():
             opt.step()
     opt = AdamW([{"params": params(), "decoupled_weight_decay": False, "weight_decay": 0.0, "maximize": False}], weight_decay=0.1)
     opt.step()
+
+
+def test_adamw_obeys_hooks_of_loading():
+    """Hooks change what is loaded before, and see and change what has been loaded after, as with torch's optimisers."""
+    from landmark_b200.optim import AdamW
+
+    p, q = (torch.nn.Parameter(torch.zeros(4, dtype=torch.bfloat16)) for _ in range(2))
+    state = {"step": 3, "exp_avg": torch.ones(4), "exp_avg_sq": torch.ones(4), "master": torch.ones(4)}
+    saved = AdamW([q]).state_dict()
+    saved["state"][0] = state
+    opt = AdamW([p])
+    seen = []
+
+    def before(_, d):
+        return {**d, "state": {0: {**d["state"][0], "step": 7}}, "param_groups": [{**d["param_groups"][0], "lr": 0.125}]}
+
+    def after(o):
+        seen.append((o.state[p]["step"], o.state[p]["exp_avg"].dtype))
+        o.state[p]["step"] = 9
+
+    handles = opt.register_load_state_dict_pre_hook(before), opt.register_load_state_dict_post_hook(after)
+    opt.load_state_dict(saved)
+    assert seen == [(7, torch.float32)] and opt.state[p]["step"] == 9 and opt.param_groups[0]["lr"] == 0.125
+    assert state["step"] == 3
+    for h in handles:
+        h.remove()
+    opt.load_state_dict(saved)
+    assert opt.state[p]["step"] == 3 and opt.state[p]["master"] is not state["master"] and len(seen) == 1
+    assert len(opt._optimizer_load_state_dict_pre_hooks) == len(opt._optimizer_load_state_dict_post_hooks) == 0
+    bad = opt.register_load_state_dict_pre_hook(lambda o, d: {**d, "param_groups": [{**d["param_groups"][0], "maximize": True}]})
+    with pytest.raises(ValueError, match="not offered"):
+        opt.load_state_dict(saved)
+    bad.remove()
+    assert len(opt._optimizer_load_state_dict_pre_hooks) == len(opt._optimizer_load_state_dict_post_hooks) == 0
