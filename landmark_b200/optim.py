@@ -44,13 +44,22 @@ def _no_capture():
                            "AdamWTensors.step_clocked() with an AdamWClock")
 
 
+def _shared(ranges) -> Optional[Tuple[str, str]]:
+    """Names of two of the ``ranges`` (address, bytes, name) that share memory, if any do."""
+    ranges = sorted(ranges)
+    for (a, size, first), (b, _, second) in zip(ranges, ranges[1:]):
+        if a + size > b:
+            return first, second
+    return None
+
+
 class AdamWTensors:
     """Parameters and optimiser states that are stepped together: checked once, then stepped with new gradients.
 
     ``params``: dense CUDA tensors of one type (float32, float16, bfloat16) on one device; ``exp_avgs`` and ``exp_avg_sqs``: the
     moments, float32 of the same sizes, or float8_e4m3fn codes with ``exp_avg_scales`` and ``exp_avg_sq_scales`` (float32, one for
-    every 256 values).  ``masters``: float32 copies of 16-bit parameters.  The tensors are updated in place where they
-    were when this was made; a step with a parameter that was given other memory since is refused."""
+    every 256 values).  ``masters``: float32 copies of 16-bit parameters.  The tensors share no memory, with each other or with the gradients;
+    they are updated in place where they were when this was made; a step with a parameter that was given other memory since is refused."""
 
     def __init__(self, params: Sequence[torch.Tensor], exp_avgs: Sequence[torch.Tensor], exp_avg_sqs: Sequence[torch.Tensor],
                  exp_avg_scales: Optional[Sequence[torch.Tensor]] = None, exp_avg_sq_scales: Optional[Sequence[torch.Tensor]] = None,
@@ -81,7 +90,7 @@ class AdamWTensors:
             self._tensors["masters"] = (list(masters), torch.float32, sizes)
         self.sizes = sizes
         self._table = np.zeros((len(sizes), _WORDS), dtype=np.int64)
-        written = set()
+        ranges = []
         for column, name in ((0, "params"), (2, "exp_avgs"), (3, "exp_avg_sqs"), (4, "exp_avg_scales"), (5, "exp_avg_sq_scales"), (6, "masters")):
             if name not in self._tensors:
                 continue
@@ -94,10 +103,12 @@ class AdamWTensors:
                 if t.dtype != dtype or t.device != self.device or t.numel() != n or t.layout is not torch.strided or not t.is_contiguous():
                     raise ValueError(f"{name}[{k}] must be {n} contiguous values of {dtype} on {self.device}, got {tuple(t.shape)} of {t.dtype} "
                                      f"on {t.device}")
-                if n and t.data_ptr() in written:
-                    raise ValueError(f"{name}[{k}] lies in the memory of another tensor of the step")
-                written.add(t.data_ptr())
                 self._table[k, column] = t.data_ptr()
+                if n:
+                    ranges.append((t.data_ptr(), n * t.element_size(), f"{name}[{k}]"))
+        shared = _shared(ranges)
+        if shared:
+            raise ValueError(f"{shared[1]} lies in the memory of another tensor of the step, {shared[0]}")
         self._table[:, _N] = sizes
         self._table[:, _N + 1] = np.arange(len(sizes))
         self.starts = self._table[:, 0].tolist()  # addresses of the parameters

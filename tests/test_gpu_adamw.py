@@ -556,3 +556,23 @@ def test_backward_over_stepped_parameters_is_refused(state_bits):
             with pytest.raises(RuntimeError, match="modified by an inplace operation"):
                 kept[0].backward()
             kept[1].backward()
+
+
+def test_tensors_that_overlap_are_refused():
+    """By part, not only from the same address on; tensors that touch are none."""
+    from landmark_b200.optim import AdamWTensors
+
+    flat = torch.zeros(1000, device="cuda")
+    m, v = ([torch.zeros(100, device="cuda") for _ in range(2)] for _ in range(2))
+    AdamWTensors([flat[:100], flat[100:200]], m, v)
+    with pytest.raises(ValueError, match=r"params\[1\] lies in the memory of another tensor of the step, params\[0\]"):
+        AdamWTensors([flat[:100], flat[99:199]], m, v)
+    with pytest.raises(ValueError, match="memory of another"):
+        AdamWTensors([flat[300:400], flat[:100]], m, [v[0], flat[350:450]])
+    AdamWTensors([flat[300:400], flat[:100], flat[320:320]], m + [m[0][:0]], v + [v[0][:0]])  # one without values lies nowhere
+    codes = torch.zeros(600, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn)
+    scales = [torch.zeros(2, device="cuda") for _ in range(2)]
+    with pytest.raises(ValueError, match="memory of another"):
+        AdamWTensors([flat[:300]], [codes[:300]], [codes[299:599]], scales[:1], scales[1:])
+    with pytest.raises(ValueError, match="memory of another"):
+        AdamWTensors([flat[:300]], [codes[:300]], [codes[300:]], scales[:1], [flat[299:301]])

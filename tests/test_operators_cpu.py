@@ -211,3 +211,15 @@ def test_adamw_obeys_hooks_of_loading():
         opt.load_state_dict(saved)
     bad.remove()
     assert len(opt._optimizer_load_state_dict_pre_hooks) == len(opt._optimizer_load_state_dict_post_hooks) == 0
+
+
+def test_shared_memory_is_found():
+    """Ranges of the tensors of a step: every pair of overlapping ones among many, neighbours that only touch are none."""
+    from landmark_b200.optim import _shared
+
+    apart = [(1000 + 16 * k, 16, k) for k in range(50)]
+    assert _shared([]) is None and _shared(apart) is None and _shared(apart[::-1]) is None
+    for k in range(50):
+        for at, size in ((1000 + 16 * k, 1), (1000 + 16 * k + 15, 1), (1000 + 16 * k + 3, 200), (1000 + 16 * k - 4, 5), (0, 10000)):
+            assert _shared(apart + [(at, size, "new")]) is not None
+    assert _shared(apart + [(1800, 4, "new"), (996, 4, "other")]) is None
