@@ -96,6 +96,21 @@ def _lookup(indices: torch.Tensor, weight: torch.Tensor, scale: float) -> torch.
     return out
 
 
+def _rows_share(a: int, a_rows: int, a_stride: int, a_bytes: int, b: int, b_rows: int, b_stride: int, b_bytes: int) -> bool:
+    """Whether rows of ``a_bytes`` at a, a + a_stride ... share memory with those at b: columns of one buffer beside each other do not."""
+    if a + (a_rows - 1) * a_stride + a_bytes <= b or b + (b_rows - 1) * b_stride + b_bytes <= a:
+        return False
+    if a_rows > b_rows:  # (the loop goes over the fewer rows)
+        a, a_rows, a_stride, a_bytes, b, b_rows, b_stride, b_bytes = b, b_rows, b_stride, b_bytes, a, a_rows, a_stride, a_bytes
+    if a_stride == b_stride:  # only the rows' distance counts: one row of a against all that b's may be beside it
+        b, b_rows, a_rows = b - (a_rows - 1) * b_stride, a_rows + b_rows - 1, 1
+    for row in range(a, a + a_rows * a_stride, a_stride) if a_rows > 1 else (a,):
+        first = max(0, (row - b - b_bytes) // b_stride + 1)  # the first row of b that ends behind the beginning of this one
+        if first < b_rows and b + first * b_stride < row + a_bytes:
+            return True
+    return False
+
+
 _workspace_bytes: dict = {}  # sizes of a call -> bytes the library asks for
 
 
@@ -111,12 +126,18 @@ def _workspace_need(n: int, rows: int, dim: int) -> int:
 
 
 def _gradient(grad: torch.Tensor, indices: torch.Tensor, scale: float, padding_idx: Optional[int], out: torch.Tensor,
-              accumulate: bool) -> torch.Tensor:
+              accumulate: bool, written: bool) -> torch.Tensor:
     kind, device, n = _kind("grad_output", grad), grad.get_device(), indices.numel()
     bits = _index_bits(indices, device)
     rows, dim = out.shape
     grad, stride = _rows(grad if grad.dim() == 2 else grad.reshape(n, dim))
     indices = indices.contiguous()
+    if written:  # `out` is the caller's: it must not be what the kernels read
+        size = out.element_size()
+        at, step, width = out.data_ptr(), (out.stride(0) if rows > 1 else dim) * size, dim * size
+        if n and (_rows_share(at, rows, step, width, grad.data_ptr(), n, stride * grad.element_size(), dim * grad.element_size())
+                  or _rows_share(at, rows, step, width, indices.data_ptr(), 1, n * bits // 8, n * bits // 8)):
+            raise ValueError("out shares memory with grad_output or indices")
     with _on(device):
         need = _workspace_need(n, rows, dim)
         ws = torch.empty(need, dtype=torch.uint8, device=grad.device) if need else None
@@ -184,7 +205,7 @@ class _EmbeddingBackward(torch.autograd.Function):
 
 
 def _new_gradient(grad, indices, num_rows, scale, padding_idx, dtype):
-    return _gradient(grad, indices, scale, padding_idx, grad.new_empty((num_rows, grad.shape[-1]), dtype=dtype), False)
+    return _gradient(grad, indices, scale, padding_idx, grad.new_empty((num_rows, grad.shape[-1]), dtype=dtype), False, False)
 
 
 def _check_padding(padding_idx: int, rows: int) -> int:
@@ -210,7 +231,8 @@ def embedding_backward(grad_output: torch.Tensor, indices: torch.Tensor, num_row
     ``grad_output[t]`` with ``indices[t] == v``, and zeros where there is none; ``grad_output [*indices.shape, dim]``.
 
     ``dtype``: the result's type (that of ``grad_output``).  ``out [num_rows, dim]``: where it is written, or with
-    ``accumulate`` added to; neighbouring values of a row next to each other.  ``padding_idx``: a row that gets nothing."""
+    ``accumulate`` added to; neighbouring values of a row next to each other, no memory shared with ``grad_output`` or ``indices``.  ``padding_idx``: a row
+    that gets nothing."""
     _kind("grad_output", grad_output)
     if grad_output.dim() != indices.dim() + 1 or grad_output.shape[:-1] != indices.shape or grad_output.shape[-1] == 0:
         raise ValueError(f"grad_output {tuple(grad_output.shape)} does not fit indices {tuple(indices.shape)}")
@@ -238,6 +260,6 @@ def embedding_backward(grad_output: torch.Tensor, indices: torch.Tensor, num_row
         raise ValueError(f"out must have neighbouring values next to each other and rows that do not overlap, got strides {out.stride()}")
     if _differentiated(grad_output) or _differentiated(out):
         raise RuntimeError("embedding_backward writes out in place and is not differentiable then")
-    _gradient(grad_output, indices, float(scale), padding_idx, out, bool(accumulate))
+    _gradient(grad_output, indices, float(scale), padding_idx, out, bool(accumulate), True)
     increment_version(out)  # a backward pass over what was computed from the old values is an error
     return out

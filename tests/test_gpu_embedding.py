@@ -408,3 +408,25 @@ def test_forward_mode_tangents():
     with torch.no_grad(), fwd.dual_level():
         idx, g, w = make(50, 40, 24, torch.float32)
         assert fwd.unpack_dual(embedding(idx, fwd.make_dual(w, g[:40]))).tangent is not None
+
+
+def test_out_that_is_read_is_refused():
+    from landmark_b200.embedding import embedding_backward
+
+    g = torch.randn((3000, 48), device="cuda")
+    idx = torch.arange(3000, device="cuda") % 40
+    kept = g.clone()
+    for accumulate in (False, True):
+        for out, rows in ((g, 3000), (g[:40], 40), (g[2960:], 40), (g.view(-1)[5:5 + 40 * 48].view(40, 48), 40)):
+            with pytest.raises(ValueError, match="shares memory"):
+                embedding_backward(g, idx, rows, out=out, accumulate=accumulate)
+    with pytest.raises(ValueError, match="shares memory"):
+        embedding_backward(g, idx, 60, out=idx.view(torch.float32)[:60 * 48].view(60, 48))
+    assert torch.equal(g, kept) and torch.equal(idx, torch.arange(3000, device="cuda") % 40)
+    wide = torch.randn((3000, 100), device="cuda")  # beside each other in one buffer: as it was
+    kept = wide.clone()
+    embedding_backward(wide[:, :48], idx, 3000, out=wide[:, 50:98])
+    check_gradient(wide[:, 50:98], kept[:, :48], idx, 3000)
+    assert torch.equal(wide[:, :50], kept[:, :50]) and torch.equal(wide[:, 98:], kept[:, 98:])
+    got = embedding_backward(g[:1].expand(3000, 48), idx, 40, out=g[1:41])  # what is copied first may lie beside
+    check_gradient(got, g[:1].expand(3000, 48), idx, 40)

@@ -223,3 +223,19 @@ def test_shared_memory_is_found():
         for at, size in ((1000 + 16 * k, 1), (1000 + 16 * k + 15, 1), (1000 + 16 * k + 3, 200), (1000 + 16 * k - 4, 5), (0, 10000)):
             assert _shared(apart + [(at, size, "new")]) is not None
     assert _shared(apart + [(1800, 4, "new"), (996, 4, "other")]) is None
+
+
+def test_rows_that_share_memory_are_found():
+    """Against sets of bytes, for all small layouts of two arrays of rows."""
+    from landmark_b200.embedding import _rows_share
+
+    def bytes_of(at, rows, stride, width):
+        return {at + r * stride + k for r in range(rows) for k in range(width)}
+
+    for a_rows, a_stride, a_width in ((1, 4, 4), (3, 4, 4), (4, 12, 4), (2, 16, 6), (5, 6, 2)):
+        for b_rows, b_stride, b_width in ((1, 2, 2), (4, 4, 4), (3, 12, 8), (2, 12, 4), (3, 16, 8), (7, 6, 4), (1, 40, 40)):
+            for b in range(100):
+                want = bool(bytes_of(50, a_rows, a_stride, a_width) & bytes_of(b, b_rows, b_stride, b_width))
+                assert _rows_share(50, a_rows, a_stride, a_width, b, b_rows, b_stride, b_width) == want
+    # columns of one wide buffer, many rows
+    assert not _rows_share(0, 10 ** 9, 800, 400, 400, 10 ** 9, 800, 400) and _rows_share(0, 10 ** 9, 800, 404, 400, 10 ** 9, 800, 400)
