@@ -583,12 +583,20 @@ int launch_table(const Table<K>& table, const Clock* clock, uint32_t blocks, int
   });
 }
 
+// Whether the tensors have 32-bit copies: as the first one with values has (one without has no addresses).
+bool has_master(const GnrAdamwTensor* tensors, int n) {
+  for (int k = 0; k < n; ++k)
+    if (tensors[k].n > 0) return tensors[k].master != nullptr;
+  return false;
+}
+
 // (`clock`: null, or where the step's numbers are instead of in `h` and `seed`)
 template <bool Clocked, int K>
 int step_all(const GnrAdamwTensor* tensors, int n, const Hyper& h, const Clock* clock, int p_type, int g_type, int bits, uint32_t seed, cudaStream_t st) {
   const int chunk = bits == 8 ? kChunk8 : kChunk;
   Table<K> table;
   table.h = h;
+  const bool master = has_master(tensors, n);
   int k = 0;
   while (k < n) {
     uint64_t blocks = 0;
@@ -604,7 +612,7 @@ int step_all(const GnrAdamwTensor* tensors, int n, const Hyper& h, const Clock* 
       blocks += need;
     }
     if (table.n > 0)
-      if (int rc = launch_table<Clocked>(table, clock, (uint32_t)blocks, p_type, g_type, tensors[0].master != nullptr, bits, st)) return rc;
+      if (int rc = launch_table<Clocked>(table, clock, (uint32_t)blocks, p_type, g_type, master, bits, st)) return rc;
   }
   return 0;
 }
@@ -614,7 +622,7 @@ int check_tensors(const char* what, const GnrAdamwTensor* tensors, int n, int pa
     gnr_set_error("%s: null pointer, unknown element type, or states of %d bits (8 or 32)", what, bits);
     return -1;
   }
-  const bool master = n > 0 && tensors[0].master != nullptr;
+  const bool master = has_master(tensors, n);
   if (master && param_type == GNR_FP32) {
     gnr_set_error("%s: fp32 parameters have no 32-bit copy", what);
     return -1;
@@ -623,7 +631,7 @@ int check_tensors(const char* what, const GnrAdamwTensor* tensors, int n, int pa
     const GnrAdamwTensor& t = tensors[k];
     if (t.n < 0 || t.n > (int64_t)0x7fffffff * (bits == 8 ? kChunk8 : kChunk) ||
         (t.n > 0 && (!t.param || !t.grad || !t.exp_avg || !t.exp_avg_sq || (bits == 8 && (!t.exp_avg_scale || !t.exp_avg_sq_scale)))) ||
-        (t.master != nullptr) != master) {
+        (t.n > 0 && (t.master != nullptr) != master)) {
       gnr_set_error("%s: tensor %d of %lld values: null pointer, or some tensors have a 32-bit copy and others none", what, k, (long long)t.n);
       return -1;
     }

@@ -576,3 +576,44 @@ def test_tensors_that_overlap_are_refused():
         AdamWTensors([flat[:300]], [codes[:300]], [codes[299:599]], scales[:1], scales[1:])
     with pytest.raises(ValueError, match="memory of another"):
         AdamWTensors([flat[:300]], [codes[:300]], [codes[300:]], scales[:1], [flat[299:301]])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("eight", [False, True])
+def test_tensors_without_values_beside_masters(dtype, eight):
+    """One without values, in first or middle place, changes nothing for 16-bit parameters with 32-bit copies; the class too."""
+    from landmark_b200.optim import AdamW, AdamWClock, AdamWTensors
+
+    for sizes in ([0, 300], [300, 0, 257], [0, 0, 5, 0]):
+        def build(n):
+            p, g, m, v, x = tensors(n, dtype, dtype)
+            scales = (None, None)
+            if eight:
+                m, v, *scales = random_states(n)
+            return AdamWTensors(p, m, v, *scales, x), g, (p, m, v, x)
+
+        keep = [k for k, n in enumerate(sizes) if n]
+        for clocked in (False, True):
+            made, g, a = build(sizes)
+            if clocked:
+                clock = AdamWClock("cuda", lr=1e-2, step=3, seed=1)
+                clock.advance()
+                made.step_clocked(g, clock)
+            else:
+                made.step(g, step=4, lr=1e-2, seed=1)
+            alone, g, b = build([sizes[k] for k in keep])
+            alone.step(g, step=4, lr=1e-2, seed=1)
+            for name, (xs, ys) in zip("pmvx", zip(a, b)):
+                for k, y in zip(keep, ys):
+                    if not eight or name in "px":  # (codes are rounded by a tensor's number)
+                        off = 0.0 if not clocked else torch.finfo(xs[k].dtype).eps * (xs[k].double().abs() + 0.1)
+                        assert bool(((xs[k].double() - y.double()).abs() <= off).all())
+    q = [torch.nn.Parameter(torch.randn(n, device="cuda").to(dtype)) for n in (0, 300, 0, 7)]
+    old = [t.detach().clone() for t in q]
+    opt = AdamW(q, lr=0.5, weight_decay=0.0, state_bits=8 if eight else 32)
+    for t in q:
+        t.grad = torch.ones_like(t)
+    opt.step()  # equal gradients: a first step is the rate
+    for t, a in zip(q, old):
+        want = a.double() - 0.5
+        assert bool(((t.double() - want).abs() <= 20 * U * (a.double().abs() + 1) + torch.finfo(dtype).eps / 2 * want.abs() * 1.001 + 2.0 ** -25).all())

@@ -239,3 +239,24 @@ def test_rows_that_share_memory_are_found():
                 assert _rows_share(50, a_rows, a_stride, a_width, b, b_rows, b_stride, b_width) == want
     # columns of one wide buffer, many rows
     assert not _rows_share(0, 10 ** 9, 800, 400, 400, 10 ** 9, 800, 400) and _rows_share(0, 10 ** 9, 800, 404, 400, 10 ** 9, 800, 400)
+
+
+def test_adamw_entry_passes_over_tensors_without_values():
+    """They have no addresses, and no say in whether the others have a 32-bit copy: what is refused is a mix among those with values."""
+    from landmark_b200 import _lib
+
+    def call(*tensors, bits=32):
+        t = (_lib.GnrAdamwTensor * len(tensors))()
+        for k, (n, master) in enumerate(tensors):
+            t[k].n = n
+            if n:
+                t[k].param = t[k].grad = t[k].exp_avg = t[k].exp_avg_sq = t[k].exp_avg_scale = t[k].exp_avg_sq_scale = 256
+            if master:
+                t[k].master = 256
+        return _lib.lib.gnr_adamw_step(t, len(tensors), _lib.BF16, _lib.BF16, bits, 1, 1e-3, 0.9, 0.999, 1e-8, 0.0, 0, None), _lib.lib.gnr_last_error()
+
+    for bits in (8, 32):
+        assert call((0, False), (0, True), bits=bits)[0] == 0  # nothing to do
+        for mix in (((10, True), (0, True), (10, False)), ((0, False), (10, True), (10, False)), ((0, True), (10, False), (0, False), (10, True))):
+            rc, why = call(*mix, bits=bits)
+            assert rc < 0 and b"tensor %d of 10 values" % (len(mix) - 1) in why
