@@ -472,7 +472,7 @@ int gnr_adamw_step(const GnrAdamwTensor* tensors_h, int n_tensors, int param_typ
 /* The same with count and rates in device memory (a clock: GNR_ADAMW_CLOCK_BYTES on an 8-byte boundary), for steps that are captured
  * into a CUDA graph.  gnr_adamw_clock_set: the steps done so far (the next is ``step`` + 1; -1: count and seed stay as they are) and
  * the rates, enqueued like a copy; gnr_adamw_clock_advance: one step further, once before the step's tensors; gnr_adamw_step_clocked: the step that the
- * clock stands at. */
+ * clock stands at.  At a count of 0, before the first advance, it changes nothing; at a later one every further call is that step once more. */
 enum { GNR_ADAMW_CLOCK_BYTES = 256 };
 int gnr_adamw_clock_set(void* clock, int64_t step, double lr, double beta1, double beta2, double eps, double weight_decay,
                         uint32_t seed, void* stream);

@@ -91,7 +91,8 @@ __host__ __device__ __forceinline__ uint32_t hash32(uint32_t i, uint32_t seed) {
 
 __host__ __device__ __forceinline__ Twice twice(double x) { return {(float)x, (float)x}; }
 
-// The numbers of a step from its rates and the betas' powers.  Before the first step: no step.
+// The numbers of a step from its rates and the betas' powers.  Before the `first` step, where the powers are 1 and the kernels return
+// at once, finite ones.
 __host__ __device__ __forceinline__ Hyper hyper_of(double lr, double beta1, double beta2, double eps, double decay, double power1, double power2, bool first) {
   Hyper h;
   h.b1 = twice(beta1);
@@ -252,6 +253,7 @@ template <typename P, typename G, bool Master> __device__ __forceinline__ bool a
 // quotients 1517 us), 60M bf16 values with fp32 copies in 300 tensors 250 us, 6.7 TB/s.
 template <typename P, typename G, bool Master, bool Clocked, int K>
 __global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__ Table<K> table, const Clock* __restrict__ clock) {
+  if (Clocked && clock->step == 0) return;  // not advanced yet: no step
   const Hyper& h = hyper_for<Clocked>(table, clock);
   const int number = find_tensor(table);
   const Tensor& t = table.t[number];
@@ -542,6 +544,7 @@ template <typename P, typename G, bool Master> struct Chunk8 {
 // root, with a way out for its range, takes as long (954 us), in a pass of its own longer (1091).
 template <typename P, typename G, bool Master, bool Clocked, int K>
 __global__ void __launch_bounds__(kThreads8, Clocked ? 4 : 5) adamw_8bit_kernel(const __grid_constant__ Table<K> table, const Clock* __restrict__ clock) {
+  if (Clocked && clock->step == 0) return;  // not advanced yet: no step
   const Hyper& h = hyper_for<Clocked>(table, clock);
   const int number = find_tensor(table);
   const Tensor& t = table.t[number];

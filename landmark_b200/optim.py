@@ -134,7 +134,8 @@ class AdamWTensors:
         self._tell_autograd(None if kept is grads else grads)
 
     def step_clocked(self, grads: Sequence[Optional[torch.Tensor]], clock: "AdamWClock"):
-        """The step that ``clock`` stands at, for capture into a CUDA graph: replays read the gradients where they lay then."""
+        """The step that ``clock`` stands at, for capture into a CUDA graph: replays read the gradients where they lay then.  A clock
+        that has done no step yet (``advance`` comes first) changes nothing."""
         if clock.device != self.device:
             raise ValueError(f"clock on {clock.device}, parameters on {self.device}")
         table, kind, kept = self._filled(grads)
@@ -223,7 +224,7 @@ class AdamWClock:
         self._rates = new
 
     def advance(self):
-        """One step further; once before the ``step_clocked`` calls of a step."""
+        """One step further; once before the ``step_clocked`` calls of a step, which without it would be the step before once more."""
         with _on(self.device.index):
             check(lib.gnr_adamw_clock_advance(self.memory.data_ptr(), _raw_stream(self.device.index)), "gnr_adamw_clock_advance")
 

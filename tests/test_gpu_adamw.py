@@ -617,3 +617,30 @@ def test_tensors_without_values_beside_masters(dtype, eight):
     for t, a in zip(q, old):
         want = a.double() - 0.5
         assert bool(((t.double() - want).abs() <= 20 * U * (a.double().abs() + 1) + torch.finfo(dtype).eps / 2 * want.abs() * 1.001 + 2.0 ** -25).all())
+
+
+@pytest.mark.parametrize("dtype,grad,master", [MIXES[0], MIXES[2]])
+@pytest.mark.parametrize("eight", [False, True])
+def test_a_clock_before_its_first_step_changes_nothing(dtype, grad, master, eight):
+    """Not the parameters by decay, not the states, whatever the gradients hold; also after the count has been set back to 0."""
+    from landmark_b200.optim import AdamWClock, AdamWTensors
+
+    p, g, m, v, x = tensors(SIZES, dtype, grad)
+    scales = [[], []]
+    if eight:
+        m, v, *scales = random_states(SIZES)
+    made = AdamWTensors(p, m, v, *(scales if eight else (None, None)), x if master else None)
+    g[3][0] = float("nan")
+    everything = p + m + v + scales[0] + scales[1] + x
+    kept = [bits(t.contiguous()).clone() for t in everything]
+    clock = AdamWClock("cuda", lr=1e-2, weight_decay=0.1)
+    made.step_clocked(g, clock)
+    clock.set(lr=0.5)
+    made.step_clocked(g, clock)
+    clock.advance()
+    clock.set(step=0)
+    made.step_clocked(g, clock)
+    assert all(torch.equal(bits(t.contiguous()), k) for t, k in zip(everything, kept))
+    clock.advance()
+    made.step_clocked(g, clock)
+    assert not torch.equal(bits(p[-1].contiguous()), kept[len(SIZES) - 1])
