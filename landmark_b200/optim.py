@@ -118,6 +118,17 @@ class AdamWTensors:
         self._written = list({id(t): t for t in (t if t._base is None else t._base for t in written)}.values())
         # the memory that the table names stays, whatever becomes of the tensors
         self._kept = [t.detach() for t in written]
+        self._borrowed = False
+
+    def _borrow_params(self):
+        """From here on the parameters' memory is theirs alone: the owner asks ``_here`` before every step."""
+        self._kept = self._kept[len(self.params):]
+        self._borrowed = True
+
+    def _here(self) -> bool:
+        """Whether the parameters lie where and as they did when they were checked (their type is the owner's to watch)."""
+        return (list(map(_address, self.params)) == self.starts and list(map(_numel, self.params)) == self.sizes
+                and all(map(_is_contiguous, self.params)))
 
     def step(self, grads: Sequence[Optional[torch.Tensor]], *, step: int, lr: float, betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
              weight_decay: float = 1e-2, seed: int = 0):
@@ -159,7 +170,7 @@ class AdamWTensors:
         """(a copy of the table with the gradients in it, their type or None where there are none, what has to stay until the launch)"""
         if len(grads) != len(self.sizes):
             raise ValueError(f"{len(grads)} gradients for {len(self.sizes)} tensors")
-        if list(map(_address, self.params)) != self.starts:
+        if not self._borrowed and list(map(_address, self.params)) != self.starts:
             raise ValueError("a parameter has been given other memory since it was checked")
         table = self._words.from_buffer_copy(self._table)
         try:  # all there and as they should be
@@ -325,14 +336,15 @@ class AdamW(torch.optim.Optimizer):
         old = self._sets.get(key)
         if old is not None:
             old_params, states, parts, made = old
-            if (len(old_params) == len(params) and all(map(operator.is_, old_params, params)) and made.starts == list(map(_address, params))
+            if (len(old_params) == len(params) and all(map(operator.is_, old_params, params)) and made._here()
                     and all(map(operator.is_, map(self.state.get, params), states))
                     and all(all(map(operator.is_, [s.get(name) for s in states], kept)) for name, kept in parts.items())):
                 return states, made
         states = [self._state_of(p) for p in params]
         parts = {n: [s.get(n) for s in states] for n in ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale", "master") if n in states[0]}
-        made = AdamWTensors([p.detach() for p in params], parts["exp_avg"], parts["exp_avg_sq"], parts.get("exp_avg_scale"), parts.get("exp_avg_sq_scale"),
+        made = AdamWTensors(params, parts["exp_avg"], parts["exp_avg_sq"], parts.get("exp_avg_scale"), parts.get("exp_avg_sq_scale"),
                             parts.get("master"))
+        made._borrow_params()
         for p, state in zip(params, states):  # (only now: what is refused leaves no state behind)
             self.state[p] = state
         self._sets[key] = (params, states, parts, made)
@@ -359,6 +371,9 @@ class AdamW(torch.optim.Optimizer):
                     with _on(key[1].index):
                         _no_capture()
                 todo.append((number, group, k, params, *self._tensors(key, params)))
+        if len(self._sets) > len(todo):  # sets of parameters that have moved, to another device say, are not looked up again
+            used = {id(tensors) for *_, tensors in todo}
+            self._sets = {key: kept for key, kept in self._sets.items() if id(kept[3]) in used or kept[3]._here()}
         for number, group, k, params, states, tensors in todo:
             counts = {s["step"] for s in states}
             for t in sorted(counts):  # one, unless a parameter had no gradient in some steps

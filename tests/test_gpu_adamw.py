@@ -644,3 +644,51 @@ def test_a_clock_before_its_first_step_changes_nothing(dtype, grad, master, eigh
     clock.advance()
     made.step_clocked(g, clock)
     assert not torch.equal(bits(p[-1].contiguous()), kept[len(SIZES) - 1])
+
+
+@pytest.mark.parametrize("state_bits", [8, 32])
+def test_memory_of_parameters_is_theirs(state_bits):
+    """What a parameter leaves behind when it moves is free at once; when it comes back, or lies otherwise, the step follows or refuses."""
+    from landmark_b200.optim import AdamW
+
+    n = 4096
+    p = torch.nn.Parameter(torch.randn(n, n, device="cuda"))
+    other = torch.nn.Parameter(torch.randn(5, device="cuda"))
+    opt = AdamW([p, other], lr=1e-2, weight_decay=0.0, state_bits=state_bits)
+    p.grad, other.grad = torch.ones_like(p), torch.ones_like(other)
+    opt.step()
+    p.grad = None
+    before = torch.cuda.memory_allocated()
+    p.data = p.data.cpu()
+    assert before - torch.cuda.memory_allocated() >= 4 * n * n
+    opt.step()  # the other goes on
+    taken = torch.full((n, n), 7.0, device="cuda")  # perhaps where the parameter was
+    p.data = p.data.cuda()
+    p.grad = torch.ones_like(p)
+    old = p.detach().clone()
+    opt.step()
+    assert float((old - p.detach() - 1e-2).abs().max()) <= (1e-6 if state_bits == 32 else 2e-3) and bool((taken == 7.0).all())
+    assert opt.state[p]["step"] == 2 and opt.state[other]["step"] == 3
+    old = p.detach().clone()
+    p.data = p.data.t()  # at the same address
+    p.grad = torch.ones(n, n, device="cuda").t()
+    with pytest.raises(ValueError, match="contiguous"):
+        opt.step()
+    assert torch.equal(p.detach(), old.t())
+
+
+def test_sets_of_parameters_that_moved_are_dropped():
+    from landmark_b200.optim import AdamW
+
+    p = [torch.nn.Parameter(torch.randn(100, device="cuda")) for _ in range(2)]
+    opt = AdamW([{"params": p[:1]}, {"params": p[1:]}])
+    for q in p:
+        q.grad = torch.ones_like(q)
+    opt.step()
+    assert len(opt._sets) == 2
+    p[0].grad = None
+    opt.step()
+    assert len(opt._sets) == 2  # without a gradient for once
+    p[0].data = p[0].data.cpu()
+    opt.step()
+    assert len(opt._sets) == 1
