@@ -30,6 +30,7 @@ BLOCK = _lib.ADAMW_BLOCK
 _CODES = torch.float8_e4m3fn
 _WORDS = C.sizeof(_lib.GnrAdamwTensor) // 8  # nine 64-bit words a tensor
 _GRAD, _N = 1, 7
+_step_of, _dtype_of = operator.itemgetter("step"), operator.attrgetter("dtype")
 _address, _numel, _get_device, _is_contiguous = torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.get_device, torch.Tensor.is_contiguous
 
 
@@ -38,8 +39,11 @@ def state_blocks(numel: int) -> int:
     return -(-numel // BLOCK)
 
 
+_capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", torch.cuda.is_current_stream_capturing)
+
+
 def _no_capture():
-    if torch.cuda.is_current_stream_capturing():
+    if _capturing():
         raise RuntimeError("an AdamW step cannot be captured into a CUDA graph: a replay would repeat this step's count and rates.  Capture "
                            "AdamWTensors.step_clocked() with an AdamWClock")
 
@@ -78,6 +82,7 @@ class AdamWTensors:
             raise ValueError("exp_avg_scales and exp_avg_sq_scales go with float8_e4m3fn states, and with no others")
         if masters is not None and self.dtype == torch.float32:
             raise ValueError("float32 parameters have no masters")
+        self._index = self.device.index
         state = _CODES if eight else torch.float32
         sizes = [p.numel() for p in self.params]
         blocks = [state_blocks(n) for n in sizes]
@@ -89,7 +94,7 @@ class AdamWTensors:
         if masters is not None:
             self._tensors["masters"] = (list(masters), torch.float32, sizes)
         self.sizes = sizes
-        self._table = np.zeros((len(sizes), _WORDS), dtype=np.int64)
+        table = np.zeros((len(sizes), _WORDS), dtype=np.int64)
         ranges = []
         for column, name in ((0, "params"), (2, "exp_avgs"), (3, "exp_avg_sqs"), (4, "exp_avg_scales"), (5, "exp_avg_sq_scales"), (6, "masters")):
             if name not in self._tensors:
@@ -103,18 +108,19 @@ class AdamWTensors:
                 if t.dtype != dtype or t.device != self.device or t.numel() != n or t.layout is not torch.strided or not t.is_contiguous():
                     raise ValueError(f"{name}[{k}] must be {n} contiguous values of {dtype} on {self.device}, got {tuple(t.shape)} of {t.dtype} "
                                      f"on {t.device}")
-                self._table[k, column] = t.data_ptr()
+                table[k, column] = t.data_ptr()
                 if n:
                     ranges.append((t.data_ptr(), n * t.element_size(), f"{name}[{k}]"))
         shared = _shared(ranges)
         if shared:
             raise ValueError(f"{shared[1]} lies in the memory of another tensor of the step, {shared[0]}")
-        self._table[:, _N] = sizes
-        self._table[:, _N + 1] = np.arange(len(sizes))
-        self.starts = self._table[:, 0].tolist()  # addresses of the parameters
-        self._words = C.c_int64 * self._table.size
+        table[:, _N] = sizes
+        table[:, _N + 1] = np.arange(len(sizes))
+        self.starts = table[:, 0].tolist()  # addresses of the parameters
+        self._words, self._bytes = C.c_int64 * table.size, table.tobytes()
         written = [t for tensors, _, _ in self._tensors.values() for t in tensors]
-        # what autograd counts the writes of: views share the count of the tensor that they are views of
+        # what autograd counts the writes of, so that a backward pass over what was computed from old values is an error: views share the
+        # count of the tensor that they are views of
         self._written = list({id(t): t for t in (t if t._base is None else t._base for t in written)}.values())
         # the memory that the table names stays, whatever becomes of the tensors
         self._kept = [t.detach() for t in written]
@@ -137,12 +143,13 @@ class AdamWTensors:
         table, kind, kept = self._filled(grads)
         if kind is None:
             return
-        index = self.device.index
+        index = self._index
         with _on(index):
-            _no_capture()
+            if not self._borrowed:  # (the owner has asked before it made the states)
+                _no_capture()
             check(lib.gnr_adamw_step(table, len(self.sizes), _TYPES[self.dtype], _TYPES[kind], self.state_bits, step, lr, betas[0], betas[1],
                                      eps, weight_decay, seed & 0xFFFFFFFF, _raw_stream(index)), "gnr_adamw_step")
-        self._tell_autograd(None if kept is grads else grads)
+        increment_version(self._written if kept is grads else self._written_with(grads))
 
     def step_clocked(self, grads: Sequence[Optional[torch.Tensor]], clock: "AdamWClock"):
         """The step that ``clock`` stands at, for capture into a CUDA graph: replays read the gradients where they lay then.  A clock
@@ -152,19 +159,14 @@ class AdamWTensors:
         table, kind, kept = self._filled(grads)
         if kind is None:
             return
-        index = self.device.index
+        index = self._index
         with _on(index):
             check(lib.gnr_adamw_step_clocked(table, len(self.sizes), _TYPES[self.dtype], _TYPES[kind], self.state_bits, clock.memory.data_ptr(),
                                              _raw_stream(index)), "gnr_adamw_step_clocked")
-        self._tell_autograd(None if kept is grads else grads)
+        increment_version(self._written if kept is grads else self._written_with(grads))
 
-    def _tell_autograd(self, grads):
-        """The step's tensors (``grads``: those that have a gradient) have been written: a backward pass over what was computed from them
-        before is an error."""
-        if grads is None:
-            increment_version(self._written)
-        else:
-            increment_version([t for tensors, _, _ in self._tensors.values() for t, g in zip(tensors, grads) if g is not None])
+    def _written_with(self, grads):
+        return [t for tensors, _, _ in self._tensors.values() for t, g in zip(tensors, grads) if g is not None]
 
     def _filled(self, grads):
         """(a copy of the table with the gradients in it, their type or None where there are none, what has to stay until the launch)"""
@@ -172,10 +174,10 @@ class AdamWTensors:
             raise ValueError(f"{len(grads)} gradients for {len(self.sizes)} tensors")
         if not self._borrowed and list(map(_address, self.params)) != self.starts:
             raise ValueError("a parameter has been given other memory since it was checked")
-        table = self._words.from_buffer_copy(self._table)
+        table = self._words.from_buffer_copy(self._bytes)
         try:  # all there and as they should be
             kinds = {g.dtype for g in grads}
-            if (list(map(_numel, grads)) == self.sizes and set(map(_get_device, grads)) == {self.device.index} and len(kinds) == 1
+            if (list(map(_numel, grads)) == self.sizes and set(map(_get_device, grads)) == {self._index} and len(kinds) == 1
                     and all(map(_is_contiguous, grads)) and kinds <= _TYPES.keys()):
                 if len(grads) > 32:
                     np.frombuffer(table, dtype=np.int64)[_GRAD::_WORDS] = list(map(_address, grads))
@@ -331,14 +333,21 @@ class AdamW(torch.optim.Optimizer):
             s["master"] = p.detach().float()
         return s
 
+    @staticmethod
+    def _kept(states, parts) -> bool:
+        try:
+            return all([all(map(operator.is_, map(operator.itemgetter(name), states), kept)) for name, kept in parts.items()])
+        except KeyError:
+            return False
+
     def _tensors(self, key, params) -> Tuple[list, AdamWTensors]:
         """States of ``params`` and the checked set of them, made again where a parameter or state has been replaced."""
         old = self._sets.get(key)
         if old is not None:
-            old_params, states, parts, made = old
+            old_params, states, parts, made = old  # parts: of every state, by name
             if (len(old_params) == len(params) and all(map(operator.is_, old_params, params)) and made._here()
                     and all(map(operator.is_, map(self.state.get, params), states))
-                    and all(all(map(operator.is_, [s.get(name) for s in states], kept)) for name, kept in parts.items())):
+                    and self._kept(states, parts)):
                 return states, made
         states = [self._state_of(p) for p in params]
         parts = {n: [s.get(n) for s in states] for n in ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale", "master") if n in states[0]}
@@ -352,7 +361,7 @@ class AdamW(torch.optim.Optimizer):
 
     @torch.no_grad()
     def step(self, closure=None):
-        if torch.cuda.is_initialized():
+        if closure is not None and torch.cuda.is_initialized():
             _no_capture()
         for group in self.param_groups:
             _check_group(group)
@@ -362,9 +371,12 @@ class AdamW(torch.optim.Optimizer):
                 loss = closure()
         todo = []  # every set of every group: states are made, and refusals raised, before anything is stepped
         for number, group in enumerate(self.param_groups):
-            sets: dict = {}
-            for p in group["params"]:
-                if p.grad is not None:
+            params = [p for p in group["params"] if p.grad is not None]
+            if len(set(map(_dtype_of, params))) == len(set(map(_get_device, params))) == 1:
+                sets = {(number, params[0].device, params[0].dtype): params}
+            else:
+                sets = {}
+                for p in params:
                     sets.setdefault((number, p.device, p.dtype), []).append(p)
             for k, (key, params) in enumerate(sets.items()):
                 if key[1].type == "cuda":
@@ -375,9 +387,9 @@ class AdamW(torch.optim.Optimizer):
             used = {id(tensors) for *_, tensors in todo}
             self._sets = {key: kept for key, kept in self._sets.items() if id(kept[3]) in used or kept[3]._here()}
         for number, group, k, params, states, tensors in todo:
-            counts = {s["step"] for s in states}
+            counts = set(map(_step_of, states))
             for t in sorted(counts):  # one, unless a parameter had no gradient in some steps
-                grads = [p.grad if len(counts) == 1 or s["step"] == t else None for p, s in zip(params, states)]
+                grads = [p.grad for p in params] if len(counts) == 1 else [p.grad if s["step"] == t else None for p, s in zip(params, states)]
                 tensors.step(grads, step=int(t) + 1, lr=float(group["lr"]), betas=group["betas"], eps=group["eps"],
                              weight_decay=group["weight_decay"], seed=self.seed + 0x3C6EF372 * (2 * number + 1) + k)
             for s in states:
