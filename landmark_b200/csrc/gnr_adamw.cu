@@ -12,7 +12,8 @@
 // the largest one, v then 2^-35.6 of it.  Codes are rounded up or down at random, with the probability that keeps
 // the mean of m and the mean of v: a step with b2 = 0.999 changes v by a thousandth of itself, a code is an eighth of v
 // wide, so rounding to nearest would never move it.  The random bits are a hash of seed, step, tensor and place (16 for m,
-// 16 for v).  A positive v is never rounded to 0, which would make its next step as large as |m| / eps.
+// 16 for v).  A positive v is never rounded to 0, which would make its next step as large as |m| / eps: where its root is below the
+// smallest code it becomes that code, which is the one place where the mean is not kept.
 // The arithmetic of the codes is in separately rounded operations (no fused multiply-add), so that the codes of equal
 // inputs are equal wherever they are computed.
 #include <cuda_fp8.h>

@@ -6,7 +6,8 @@ same groups.  A step is one launch for each parameter type of a group (per 400 t
 
 8-bit states: every 256 values of a tensor share two scales; the first moment is ``scale * code``, the second
 ``(scale * code) ** 2`` with float8_e4m3fn codes, rounded at random without bias (a hash of seed, step, tensor and place, so a
-step repeats bit for bit).  A gradient that is not finite spoils its own value only.
+step repeats bit for bit); a second moment below the smallest code's, 2^-36 of the largest beside it, becomes that code, never 0.  A gradient
+that is not finite spoils its own value only.
 
 16-bit parameters can have a copy in fp32 (``masters``): the step updates the copy, the parameter is its rounded image.  Without
 one, what a step changes by less than half a unit of the last place is lost.

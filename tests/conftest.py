@@ -19,3 +19,11 @@ def built_library():
     from landmark_b200.build import build_library
 
     return build_library()
+
+
+@pytest.fixture(autouse=True)
+def _seeded():
+    """What a test draws without a seed of its own is the same in every run."""
+    import torch
+
+    torch.manual_seed(0)

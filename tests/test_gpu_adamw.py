@@ -692,3 +692,30 @@ def test_sets_of_parameters_that_moved_are_dropped():
     p[0].data = p[0].data.cpu()
     opt.step()
     assert len(opt._sets) == 1
+
+
+def test_8bit_rounding_of_every_size():
+    """The mean of the codes over 1024 seeds, as above, for values from the largest of their block down to far below the smallest code: m is
+    kept down to nothing; v is kept where its root is one code (2^-9) or more, and below, where 0 is no choice, it is that code in every case
+    (2^-18 of the scale's square, less than v's own rounding beside the largest)."""
+    from landmark_b200.optim import adamw_step
+
+    n, seeds = 1024, 1024
+    y = 448.0 * 2.0 ** (-24.0 * torch.arange(n, device="cuda") / n)  # spread over four blocks, each beginning with the largest
+    g = y.view(256, 4).t().reshape(-1).clone()
+    g[::BLOCK] = 448.0
+    p = torch.zeros(n, device="cuda")
+    m_sum, v_sum = torch.zeros(n, dtype=torch.float64, device="cuda"), torch.zeros(n, dtype=torch.float64, device="cuda")
+    for seed in range(seeds):
+        (m, v), (ms, vs) = fresh_8bit(n)
+        adamw_step([p], [g], [m], [v], step=1, lr=0.0, exp_avg_scales=[ms], exp_avg_sq_scales=[vs], seed=seed)
+        m_sum += m.double()
+        v_sum += v.double() ** 2
+    allowed = 6 * 0.5 / math.sqrt(seeds) + 2.0 ** -17
+    y = g.double()  # in units of the scale: the block's largest is 448
+    width = torch.exp2(torch.floor(torch.log2(y.clamp(2.0 ** -6, 447.9)))) / 8
+    assert bool(((m_sum / seeds - y).abs() <= allowed * width + 1e-6 * y).all())
+    small = y < 2.0 ** -9
+    assert 100 < int(small.sum()) < 400
+    assert bool((v_sum[small] == seeds * 2.0 ** -18).all())
+    assert bool(((v_sum / seeds - y * y).abs() <= allowed * (2 * y + width) * width + 1e-6 * y * y)[~small].all())
