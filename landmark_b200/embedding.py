@@ -72,6 +72,8 @@ def _index_bits(indices: torch.Tensor, index: int) -> int:
 
 def _rows(t: torch.Tensor):
     """``t [n, d]`` with neighbouring values next to each other and rows that do not overlap, and the rows' distance."""
+    if t.is_neg():  # a view with its sign to come, as the imaginary part of a conjugate
+        t = t.resolve_neg()
     if t.is_contiguous():
         return t, t.shape[1]
     if t.shape[0] > 1 and (t.stride(1) == 1 or t.shape[1] == 1) and t.stride(0) >= t.shape[1]:
@@ -256,7 +258,7 @@ def embedding_backward(grad_output: torch.Tensor, indices: torch.Tensor, num_row
         raise TypeError(f"out is {out.dtype}, dtype {dtype}")
     if tuple(out.shape) != (num_rows, grad_output.shape[-1]) or out.device != grad_output.device:
         raise ValueError(f"out {tuple(out.shape)} on {out.device} must be {(num_rows, grad_output.shape[-1])} on {grad_output.device}")
-    if (out.stride(1) != 1 and out.shape[1] > 1) or (num_rows > 1 and out.stride(0) < out.shape[1]):
+    if out.is_neg() or (out.stride(1) != 1 and out.shape[1] > 1) or (num_rows > 1 and out.stride(0) < out.shape[1]):
         raise ValueError(f"out must have neighbouring values next to each other and rows that do not overlap, got strides {out.stride()}")
     if _differentiated(grad_output) or _differentiated(out):
         raise RuntimeError("embedding_backward writes out in place and is not differentiable then")

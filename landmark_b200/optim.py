@@ -6,7 +6,7 @@ same groups.  A step is one launch for each parameter type of a group (per 400 t
 
 8-bit states: every 256 values of a tensor share two scales; the first moment is ``scale * code``, the second
 ``(scale * code) ** 2`` with float8_e4m3fn codes, rounded at random without bias (a hash of seed, step, tensor and place, so a
-step repeats bit for bit); a second moment below the smallest code's, 2^-36 of the largest beside it, becomes that code, never 0.  A gradient
+step repeats bit for bit); a second moment below the smallest code's, 2^-35.6 of the largest beside it, becomes that code, never 0.  A gradient
 that is not finite spoils its own value only.
 
 16-bit parameters can have a copy in fp32 (``masters``): the step updates the copy, the parameter is its rounded image.  Without
@@ -84,6 +84,7 @@ class AdamWTensors:
         if masters is not None and self.dtype == torch.float32:
             raise ValueError("float32 parameters have no masters")
         self._index = self.device.index
+        self._single = [k for k, p in enumerate(self.params) if p.numel() == 1]  # a view with its sign to come is contiguous only there
         state = _CODES if eight else torch.float32
         sizes = [p.numel() for p in self.params]
         blocks = [state_blocks(n) for n in sizes]
@@ -106,7 +107,7 @@ class AdamWTensors:
             for k, (t, n) in enumerate(zip(tensors, want)):
                 if not isinstance(t, torch.Tensor):
                     raise TypeError(f"{name}[{k}] must be a tensor, got {type(t).__name__}")
-                if t.dtype != dtype or t.device != self.device or t.numel() != n or t.layout is not torch.strided or not t.is_contiguous():
+                if t.dtype != dtype or t.device != self.device or t.numel() != n or t.layout is not torch.strided or not t.is_contiguous() or t.is_neg():
                     raise ValueError(f"{name}[{k}] must be {n} contiguous values of {dtype} on {self.device}, got {tuple(t.shape)} of {t.dtype} "
                                      f"on {t.device}")
                 table[k, column] = t.data_ptr()
@@ -179,7 +180,7 @@ class AdamWTensors:
         try:  # all there and as they should be
             kinds = {g.dtype for g in grads}
             if (list(map(_numel, grads)) == self.sizes and set(map(_get_device, grads)) == {self._index} and len(kinds) == 1
-                    and all(map(_is_contiguous, grads)) and kinds <= _TYPES.keys()):
+                    and all(map(_is_contiguous, grads)) and kinds <= _TYPES.keys() and not any([grads[k].is_neg() for k in self._single])):
                 if len(grads) > 32:
                     np.frombuffer(table, dtype=np.int64)[_GRAD::_WORDS] = list(map(_address, grads))
                 else:
@@ -204,7 +205,7 @@ class AdamWTensors:
                 kind = g.dtype
             if g.dtype is not kind or kind not in _TYPES:
                 raise TypeError(f"gradients must be of one type, float32, float16 or bfloat16: got {g.dtype} at {k}, {kind} before")
-            g = g.contiguous()
+            g = g.contiguous().resolve_neg()
             kept.append(g)
             table[k * _WORDS + _GRAD] = g.data_ptr()
         return kept, kind

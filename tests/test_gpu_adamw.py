@@ -719,3 +719,17 @@ def test_8bit_rounding_of_every_size():
     assert 100 < int(small.sum()) < 400
     assert bool((v_sum[small] == seeds * 2.0 ** -18).all())
     assert bool(((v_sum / seeds - y * y).abs() <= allowed * (2 * y + width) * width + 1e-6 * y * y)[~small].all())
+
+
+def test_gradients_with_their_sign_to_come():
+    """The imaginary part of a conjugate is read with its sign; as a parameter it is refused."""
+    from landmark_b200.optim import AdamWTensors
+
+    for n in (1, 200):
+        z = torch.randn(n, dtype=torch.complex64, device="cuda").conj()
+        p, m, v = torch.zeros(n, device="cuda"), torch.zeros(n, device="cuda"), torch.zeros(n, device="cuda")
+        assert z.imag.is_neg()
+        AdamWTensors([p], [m], [v]).step([z.imag], step=1, lr=0.25, weight_decay=0.0)
+        assert torch.equal(torch.sign(p), -torch.sign(z.imag)) and torch.equal(torch.sign(m), torch.sign(z.imag))
+        with pytest.raises(ValueError, match="contiguous"):
+            AdamWTensors([z.imag], [m], [v])

@@ -430,3 +430,20 @@ def test_out_that_is_read_is_refused():
     assert torch.equal(wide[:, :50], kept[:, :50]) and torch.equal(wide[:, 98:], kept[:, 98:])
     got = embedding_backward(g[:1].expand(3000, 48), idx, 40, out=g[1:41])  # what is copied first may lie beside
     check_gradient(got, g[:1].expand(3000, 48), idx, 40)
+
+
+def test_imaginary_parts_of_conjugates():
+    """Views whose sign is still to come: read with it, refused where they are written."""
+    from landmark_b200.embedding import embedding, embedding_backward
+
+    idx, _, _ = make(500, 40, 1, torch.float32)
+    z = torch.randn((500, 1), dtype=torch.complex64, device="cuda").conj()
+    g, w = z.imag, z[:40].imag
+    assert g.is_neg() and w.is_neg()
+    assert torch.equal(embedding(idx, w), w[idx])
+    check_gradient(embedding_backward(g, idx, 40), g, idx, 40)
+    wide = torch.randn((500, 24), dtype=torch.complex64, device="cuda").conj().imag
+    assert torch.equal(embedding(idx, wide[:40]), wide[:40][idx])
+    check_gradient(embedding_backward(wide, idx, 40), wide, idx, 40)
+    with pytest.raises(ValueError, match="out must"):
+        embedding_backward(z.imag.clone(), idx, 40, out=w)
