@@ -92,8 +92,7 @@ __host__ __device__ __forceinline__ uint32_t hash32(uint32_t i, uint32_t seed) {
 
 __host__ __device__ __forceinline__ Twice twice(double x) { return {(float)x, (float)x}; }
 
-// The numbers of a step from its rates and the betas' powers.  Before the `first` step, where the powers are 1 and the kernels return
-// at once, finite ones.
+// The numbers of a step from its rates and the betas' powers.  Before the `first` step, where the powers are 1: no step, told by c2_inv = 0.
 __host__ __device__ __forceinline__ Hyper hyper_of(double lr, double beta1, double beta2, double eps, double decay, double power1, double power2, bool first) {
   Hyper h;
   h.b1 = twice(beta1);
@@ -102,7 +101,7 @@ __host__ __device__ __forceinline__ Hyper hyper_of(double lr, double beta1, doub
   h.b2c = twice(1.0 - beta2);
   h.keep = twice(1.0 - lr * decay);
   h.rate = twice(first ? 0.0 : -lr / (1.0 - power1));
-  h.c2_inv = twice(first ? 1.0 : 1.0 / sqrt(1.0 - power2));
+  h.c2_inv = twice(first ? 0.0 : 1.0 / sqrt(1.0 - power2));
   h.eps = twice(eps);
   h.minus_one = twice(-1.0);
   h.two = twice(2.0);
@@ -254,8 +253,8 @@ template <typename P, typename G, bool Master> __device__ __forceinline__ bool a
 // quotients 1517 us), 60M bf16 values with fp32 copies in 300 tensors 250 us, 6.7 TB/s.
 template <typename P, typename G, bool Master, bool Clocked, int K>
 __global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__ Table<K> table, const Clock* __restrict__ clock) {
-  if (Clocked && clock->step == 0) return;  // not advanced yet: no step
   const Hyper& h = hyper_for<Clocked>(table, clock);
+  if (Clocked && h.c2_inv.x == 0.0f) return;  // not advanced yet: no step
   const int number = find_tensor(table);
   const Tensor& t = table.t[number];
   const int64_t begin = (int64_t)(blockIdx.x - table.first[number]) * kChunk;
@@ -545,8 +544,8 @@ template <typename P, typename G, bool Master> struct Chunk8 {
 // root, with a way out for its range, takes as long (954 us), in a pass of its own longer (1091).
 template <typename P, typename G, bool Master, bool Clocked, int K>
 __global__ void __launch_bounds__(kThreads8, Clocked ? 4 : 5) adamw_8bit_kernel(const __grid_constant__ Table<K> table, const Clock* __restrict__ clock) {
-  if (Clocked && clock->step == 0) return;  // not advanced yet: no step
   const Hyper& h = hyper_for<Clocked>(table, clock);
+  if (Clocked && h.c2_inv.x == 0.0f) return;  // not advanced yet: no step
   const int number = find_tensor(table);
   const Tensor& t = table.t[number];
   const int64_t first = (int64_t)(blockIdx.x - table.first[number]) * kChunk8;
