@@ -32,7 +32,16 @@ _CODES = torch.float8_e4m3fn
 _WORDS = C.sizeof(_lib.GnrAdamwTensor) // 8  # nine 64-bit words a tensor
 _GRAD, _N = 1, 7
 _step_of, _dtype_of = operator.itemgetter("step"), operator.attrgetter("dtype")
+_version_of = operator.attrgetter("_version")
 _address, _numel, _get_device, _is_contiguous = torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.get_device, torch.Tensor.is_contiguous
+
+
+def _versions(tensors) -> Optional[List[int]]:
+    """How often autograd has counted a write of each (None: of inference tensors)."""
+    try:
+        return list(map(_version_of, tensors))
+    except RuntimeError:
+        return None
 
 
 def state_blocks(numel: int) -> int:
@@ -127,6 +136,7 @@ class AdamWTensors:
         # the memory that the table names stays, whatever becomes of the tensors
         self._kept = [t.detach() for t in written]
         self._borrowed = False
+        self.versions: Optional[List[int]] = None  # of the parameters, after the last step
 
     def _borrow_params(self):
         """From here on the parameters' memory is theirs alone: the owner asks ``_here`` before every step."""
@@ -264,8 +274,9 @@ class AdamW(torch.optim.Optimizer):
     """``torch.optim.AdamW`` over dense CUDA parameters: groups, learning rate schedulers and ``state_dict`` as there.  Groups that
     ask for ``maximize``, ``amsgrad``, ``differentiable`` or coupled weight decay are refused.
 
-    ``state_bits``: 32 or 8.  ``master_weights``: 16-bit parameters keep an fp32 copy in the state.  ``seed``: of the random
-    rounding of 8-bit states."""
+    ``state_bits``: 32 or 8.  ``master_weights``: 16-bit parameters keep an fp32 copy in the state; what others write to a parameter
+    between steps (weights that are loaded, not writes through ``.data``, which nothing counts) is taken over into the copy.  ``seed``: of
+    the random rounding of 8-bit states."""
 
     def __init__(self, params, lr: float = 1e-3, betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2,
                  state_bits: int = 32, master_weights: bool = True, seed: int = 0):
@@ -342,6 +353,17 @@ class AdamW(torch.optim.Optimizer):
         except KeyError:
             return False
 
+    def _take_over(self, made: AdamWTensors, old):
+        """Brings the fp32 copies of parameters that others have written since the last step (weights that were loaded, say) to what they
+        hold now: a value that is still the copy's rounded image keeps its copy."""
+        now = _versions(made.params)
+        if now is None or (old is made and now == made.versions):
+            return
+        known = {} if old is None or old.versions is None else {id(p): at for p, *at in zip(old.params, old.starts, old.versions)}
+        for p, at, version, master in zip(made.params, made.starts, now, made._tensors["masters"][0]):
+            if known.get(id(p)) != [at, version]:
+                master.copy_(torch.where(p == master.to(p.dtype), master, p.float()))
+
     def _tensors(self, key, params) -> Tuple[list, AdamWTensors]:
         """States of ``params`` and the checked set of them, made again where a parameter or state has been replaced."""
         old = self._sets.get(key)
@@ -350,6 +372,8 @@ class AdamW(torch.optim.Optimizer):
             if (len(old_params) == len(params) and all(map(operator.is_, old_params, params)) and made._here()
                     and all(map(operator.is_, map(self.state.get, params), states))
                     and self._kept(states, parts)):
+                if "master" in parts:
+                    self._take_over(made, made)
                 return states, made
         states = [self._state_of(p) for p in params]
         parts = {n: [s.get(n) for s in states] for n in ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale", "master") if n in states[0]}
@@ -358,6 +382,8 @@ class AdamW(torch.optim.Optimizer):
         made._borrow_params()
         for p, state in zip(params, states):  # (only now: what is refused leaves no state behind)
             self.state[p] = state
+        if "master" in parts:
+            self._take_over(made, old[3] if old is not None else None)
         self._sets[key] = (params, states, parts, made)
         return states, made
 
@@ -396,4 +422,7 @@ class AdamW(torch.optim.Optimizer):
                              weight_decay=group["weight_decay"], seed=self.seed + 0x3C6EF372 * (2 * number + 1) + k)
             for s in states:
                 s["step"] += 1
+        for *_, tensors in todo:  # (behind all steps: parameters may share a count of writes)
+            if "masters" in tensors._tensors:
+                tensors.versions = _versions(tensors.params)
         return loss

@@ -733,3 +733,54 @@ def test_gradients_with_their_sign_to_come():
         assert torch.equal(torch.sign(p), -torch.sign(z.imag)) and torch.equal(torch.sign(m), torch.sign(z.imag))
         with pytest.raises(ValueError, match="contiguous"):
             AdamWTensors([z.imag], [m], [v])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_weights_loaded_between_steps_are_kept(dtype):
+    """What is written to a 16-bit parameter between steps is where its next step starts, whichever way it was written; values that nobody
+    wrote go on from their fp32 copies, as they do in a twin that is left alone."""
+    from landmark_b200.optim import AdamW
+
+    def build():
+        torch.manual_seed(6)
+        p = [torch.nn.Parameter(torch.randn(n, device="cuda").to(dtype)) for n in (300, 40)]
+        return p, AdamW(p, lr=1e-3, weight_decay=0.0)
+
+    def step(p, opt, t):
+        for k, q in enumerate(p):
+            q.grad = None if k == 1 and t == 2 else torch.randn(q.shape, generator=torch.Generator(device="cuda").manual_seed(10 * t + k), device="cuda").to(dtype)
+        opt.step()
+
+    new = torch.full((300,), 3.0, dtype=dtype, device="cuda")
+    flat = torch.nn.Parameter(new.clone())
+
+    def loaded(q):
+        with torch.no_grad():
+            q.copy_(new)
+
+    def part(q):
+        with torch.no_grad():
+            q[:100] = new[:100]
+
+    def replaced(q):
+        q.data = flat.detach()
+
+    for t0 in (1, 2, 3):  # before the step where the set changes, and after
+        for write, written in ((loaded, 300), (part, 100), (replaced, 300)):
+            (p, opt), (q, twin) = build(), build()
+            for t in range(5):
+                if t == t0:
+                    write(p[0])
+                    start = p[0].detach().clone()
+                step(p, opt, t)
+                step(q, twin, t)
+                if t == t0:
+                    m, v = (opt.state[p[0]][k].double() for k in ("exp_avg", "exp_avg_sq"))
+                    update = 1e-3 / (1 - 0.9 ** (t + 1)) * m / (torch.sqrt(v) / math.sqrt(1 - 0.999 ** (t + 1)) + 1e-8)
+                    want = (start.double() - update)[:written]
+                    assert bool(((opt.state[p[0]]["master"].double()[:written] - want).abs() <= 20 * U * (want.abs() + 1)).all())
+                assert torch.equal(p[0], opt.state[p[0]]["master"].to(dtype))
+                if t < t0 or write is part:
+                    assert torch.equal(opt.state[p[0]]["master"][100:], twin.state[q[0]]["master"][100:])
+                assert torch.equal(p[1], q[1]) and torch.equal(opt.state[p[1]]["master"], twin.state[q[1]]["master"])
+            flat.data = new.clone()
