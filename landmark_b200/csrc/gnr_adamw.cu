@@ -15,7 +15,8 @@
 // 16 for v).  A positive v is never rounded to 0, which would make its next step as large as |m| / eps: where its root is below the
 // smallest code it becomes that code, which is the one place where the mean is not kept.
 // The arithmetic of the codes is in separately rounded operations (no fused multiply-add), so that the codes of equal
-// inputs are equal wherever they are computed.
+// inputs are equal wherever they are computed with the same 448 / (largest in the block): here that quotient is the exact reciprocal's
+// but for some blocks in a million (scale_up).
 #include <cuda_fp8.h>
 #include <math.h>
 #include <string.h>
@@ -407,7 +408,8 @@ template <typename X, typename G> struct Part {
   float m_scale, v_scale;
 };
 
-// 448 / top, 0 for 0: the quick reciprocal and one Newton step (rounded like the exact one but for some in a million)
+// 448 / top, 0 for 0: the quick reciprocal and one Newton step (rounded like the exact one but for some in a million, where a value on the
+// border of two codes may get the other one; the exact one in every case takes 335M values 976 instead of 969 us)
 __device__ __forceinline__ float scale_up(float top) {
   if (top > 1e30f) return __fmul_rn(__frcp_rn(top), kTop);
   const float r = quick_rcp(top);
@@ -539,8 +541,10 @@ template <typename P, typename G, bool Master> struct Chunk8 {
 
 // A warp takes one block of 256 values.  Bound by its instructions, 89 a value with the packed fp32 ones counted for two (87 % of the issue
 // slots), and by the power they draw: 335M fp32 values take 966 us at 1965 MHz, 5.6 TB/s, and 1040 to 1140 us in a long run, where the power
-// cap holds the clock at 1.65 to 1.75 GHz.  Five thread blocks to an SM hide the loads better than a longer run of blocks with the
-// next one's loads ahead of the work (1058 against 948 us on zeros), six spill (1000).  A root by Newton's step from the quick reciprocal
+// cap holds the clock at 1.65 to 1.75 GHz.  Five thread blocks to an SM (48 registers, of which 24 to 36 bytes a thread spill) hide the
+// loads better than a longer run of blocks with the next one's loads ahead of the work (1058 against 948 us on zeros), six spill more (1000).
+// By a clock four (64 registers, 36 to 68 bytes spill): five would take those 335M values 1154 instead of 1206 us, but 9M unaligned bf16
+// values with fp32 copies, the form of single accesses, 57 instead of 45.  A root by Newton's step from the quick reciprocal
 // root, with a way out for its range, takes as long (954 us), in a pass of its own longer (1091).
 template <typename P, typename G, bool Master, bool Clocked, int K>
 __global__ void __launch_bounds__(kThreads8, Clocked ? 4 : 5) adamw_8bit_kernel(const __grid_constant__ Table<K> table, const Clock* __restrict__ clock) {

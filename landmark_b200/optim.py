@@ -32,7 +32,7 @@ _CODES = torch.float8_e4m3fn
 _WORDS = C.sizeof(_lib.GnrAdamwTensor) // 8  # nine 64-bit words a tensor
 _GRAD, _N = 1, 7
 _step_of, _dtype_of = operator.itemgetter("step"), operator.attrgetter("dtype")
-_version_of = operator.attrgetter("_version")
+_version_of, _layout_of, _is_neg = operator.attrgetter("_version"), operator.attrgetter("layout"), torch.Tensor.is_neg
 _address, _numel, _get_device, _is_contiguous = torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.get_device, torch.Tensor.is_contiguous
 
 
@@ -58,12 +58,12 @@ def _no_capture():
                            "AdamWTensors.step_clocked() with an AdamWClock")
 
 
-def _shared(ranges) -> Optional[Tuple[str, str]]:
-    """Names of two of the ``ranges`` (address, bytes, name) that share memory, if any do."""
+def _shared(ranges) -> Optional[tuple]:
+    """Names of two of the ``ranges`` (address, bytes, name ...) that share memory, if any do."""
     ranges = sorted(ranges)
-    for (a, size, first), (b, _, second) in zip(ranges, ranges[1:]):
-        if a + size > b:
-            return first, second
+    for one, next_one in zip(ranges, ranges[1:]):
+        if one[0] + one[1] > next_one[0]:
+            return one[2:], next_one[2:]
     return None
 
 
@@ -93,9 +93,9 @@ class AdamWTensors:
         if masters is not None and self.dtype == torch.float32:
             raise ValueError("float32 parameters have no masters")
         self._index = self.device.index
-        self._single = [k for k, p in enumerate(self.params) if p.numel() == 1]  # a view with its sign to come is contiguous only there
         state = _CODES if eight else torch.float32
         sizes = [p.numel() for p in self.params]
+        self._single = [k for k, n in enumerate(sizes) if n == 1]  # a view with its sign to come is contiguous only there
         blocks = [state_blocks(n) for n in sizes]
         self._tensors = {"params": (self.params, self.dtype, sizes), "exp_avgs": (list(exp_avgs), state, sizes),
                          "exp_avg_sqs": (list(exp_avg_sqs), state, sizes)}
@@ -113,18 +113,21 @@ class AdamWTensors:
             tensors, dtype, want = self._tensors[name]
             if len(tensors) != len(sizes):
                 raise ValueError(f"{len(tensors)} {name} for {len(sizes)} params")
-            for k, (t, n) in enumerate(zip(tensors, want)):
-                if not isinstance(t, torch.Tensor):
-                    raise TypeError(f"{name}[{k}] must be a tensor, got {type(t).__name__}")
-                if t.dtype != dtype or t.device != self.device or t.numel() != n or t.layout is not torch.strided or not t.is_contiguous() or t.is_neg():
-                    raise ValueError(f"{name}[{k}] must be {n} contiguous values of {dtype} on {self.device}, got {tuple(t.shape)} of {t.dtype} "
-                                     f"on {t.device}")
-                table[k, column] = t.data_ptr()
-                if n:
-                    ranges.append((t.data_ptr(), n * t.element_size(), f"{name}[{k}]"))
+            if not self._as_wanted(tensors, dtype, want):
+                for k, (t, n) in enumerate(zip(tensors, want)):
+                    if not isinstance(t, torch.Tensor):
+                        raise TypeError(f"{name}[{k}] must be a tensor, got {type(t).__name__}")
+                    if not self._as_wanted([t], dtype, [n]):
+                        raise ValueError(f"{name}[{k}] must be {n} contiguous values of {dtype} on {self.device}, got {tuple(t.shape)} of {t.dtype} "
+                                         f"on {t.device}")
+            addresses = list(map(_address, tensors))
+            table[:, column] = addresses
+            width = tensors[0].element_size()
+            ranges += [(at, n * width, name, k) for k, (at, n) in enumerate(zip(addresses, want)) if n]
         shared = _shared(ranges)
         if shared:
-            raise ValueError(f"{shared[1]} lies in the memory of another tensor of the step, {shared[0]}")
+            (first, i), (second, k) = shared
+            raise ValueError(f"{second}[{k}] lies in the memory of another tensor of the step, {first}[{i}]")
         table[:, _N] = sizes
         table[:, _N + 1] = np.arange(len(sizes))
         self.starts = table[:, 0].tolist()  # addresses of the parameters
@@ -137,6 +140,13 @@ class AdamWTensors:
         self._kept = [t.detach() for t in written]
         self._borrowed = False
         self.versions: Optional[List[int]] = None  # of the parameters, after the last step
+
+    def _as_wanted(self, tensors, dtype, sizes) -> bool:
+        try:
+            return (list(map(_numel, tensors)) == sizes and set(map(_dtype_of, tensors)) == {dtype} and set(map(_get_device, tensors)) == {self._index}
+                    and set(map(_layout_of, tensors)) == {torch.strided} and all(map(_is_contiguous, tensors)) and not any(map(_is_neg, tensors)))
+        except (AttributeError, TypeError, RuntimeError):
+            return False
 
     def _borrow_params(self):
         """From here on the parameters' memory is theirs alone: the owner asks ``_here`` before every step."""
