@@ -441,14 +441,14 @@ int gnr_embedding_lookup(const void* table, int type, int64_t rows, int dim, int
 /* Its gradient: out[v] = round(scale * sum of grad[t] over the t with indices[t] == v), for every row v of ``rows``; with
  * ``accumulate`` added to what out holds (rows that no index names are then not touched).  Sums in fp32, in an order that only
  * the inputs decide.  Masked places, indices past the table and those equal to ``padding_row`` (-1: none) are left out, their
- * rows of ``grad`` not read.  ``workspace`` on a 16-byte boundary, its contents are scratch. */
+ * rows of ``grad`` not read.  ``workspace`` on a 16-byte boundary, its contents are scratch.  ``out`` shares no memory with the others. */
 int gnr_embedding_grad_workspace_bytes(int64_t n, int64_t rows, int dim, size_t* bytes_h);
 int gnr_embedding_grad(const void* grad, int grad_type, int dim, int64_t grad_stride, const void* indices, int index_bits,
                        int64_t n, int64_t rows, int64_t padding_row, float scale, int accumulate, void* out, int out_type,
                        int64_t out_stride, void* workspace, size_t workspace_bytes, void* stream);
 
 /* One tensor of an optimiser step; all pointers are device pointers to dense arrays of ``n`` values (scales: of
- * ceil(n / GNR_ADAMW_BLOCK)). */
+ * ceil(n / GNR_ADAMW_BLOCK)).  They share no memory; a tensor without values needs no pointers. */
 enum { GNR_ADAMW_BLOCK = 256 }; /* values that share the scales of the 8-bit states */
 typedef struct GnrAdamwTensor {
   void* param;
