@@ -539,7 +539,7 @@ template <typename P, typename G, bool Master> struct Chunk8 {
   }
 };
 
-// A warp takes one block of 256 values.  Bound by its instructions, 89 a value with the packed fp32 ones counted for two (87 % of the issue
+// A warp takes one block of 256 values.  Bound by its instructions, 89 a value with the packed fp32 ones counted for two (86 % of the issue
 // slots), and by the power they draw: 335M fp32 values take 966 us at 1965 MHz, 5.6 TB/s, and 1040 to 1140 us in a long run, where the power
 // cap holds the clock at 1.65 to 1.75 GHz.  Five thread blocks to an SM (48 registers, of which 24 to 36 bytes a thread spill) hide the
 // loads better than a longer run of blocks with the next one's loads ahead of the work (1058 against 948 us on zeros), six spill more (1000).
